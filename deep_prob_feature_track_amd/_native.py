@@ -8,7 +8,7 @@ load, every call raises.
 import ctypes
 import os
 
-import torch  # noqa: F401  (must be imported before the HIP library, see above)
+import torch  # (must be imported before the HIP library, see above)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libdpft_ic.so")
@@ -24,6 +24,9 @@ EXTREMA_READY = 0x10000
 GROUP_SHIFT = 20          # DPFT_GROUP(n) = n << 20: n pairs per independent batch (bits 20-31)
 GROUP_MAX_BATCHES = 32
 STATUS_NONFINITE = 0x1
+GN_PACKED = 0x1
+ACTS = {"none": 0, "relu": 1, "elu": 2, "silu": 3}  # DPFT_ACT_*
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}  # DPFT_TYPE_*
 CTRL_BYTES = 20480        # the workspace's control area (counters): zero before first use (kCtrlBytes)
 ABI_VERSION = 2
 
@@ -45,10 +48,20 @@ class LevelTensors(ctypes.Structure):
     ]
 
 
+class GroupNorm(ctypes.Structure):
+    _fields_ = [
+        ("pixels", ctypes.c_int64), ("N", ctypes.c_int32), ("C", ctypes.c_int32), ("groups", ctypes.c_int32),
+        ("act", ctypes.c_int32), ("x_type", ctypes.c_int32), ("param_type", ctypes.c_int32),
+        ("flags", ctypes.c_uint32), ("eps", ctypes.c_float),
+    ]
+
+
 EXPORTS = ("dpft_workspace_size", "dpft_ic_solve_level", "dpft_ic_solve_pyramid", "dpft_ic_iterate", "dpft_ic_residual_level",
            "dpft_residual_poses_workspace_size", "dpft_ic_residual_poses", "dpft_ic_residual_map",
            "dpft_ic_reduce_only", "dpft_ic_debug_pixels", "dpft_preprocess_workspace_size",
-           "dpft_preprocess_depth", "dpft_pack_features", "dpft_pack_features_nhwc", "dpft_bn_elu", "dpft_bn_elu_pack", "dpft_sigma_extrema_levels", "dpft_ic_damped_update", "dpft_feature_gradient", "dpft_warp_jacobian",
+           "dpft_preprocess_depth", "dpft_pack_features", "dpft_pack_features_nhwc", "dpft_bn_elu", "dpft_bn_elu_pack", "dpft_sigma_extrema_levels", "dpft_ic_damped_update",
+           "dpft_group_norm_workspace_size", "dpft_group_norm_act", "dpft_group_norm_act_backward",
+           "dpft_act_checkpoint", "dpft_act_restore", "dpft_feature_gradient", "dpft_warp_jacobian",
            "dpft_inverse_jacobian", "dpft_normal_equations_workspace_size", "dpft_normal_equations",
            "dpft_read_probe_out_floats", "dpft_read_probe", "dpft_copy_probe", "dpft_version", "dpft_last_error")
 
@@ -100,6 +113,16 @@ def lib():
     L.dpft_bn_elu.restype = ctypes.c_int
     L.dpft_bn_elu_pack.argtypes = [vp, vp, vp, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, ctypes.c_int32, vp]
     L.dpft_bn_elu_pack.restype = ctypes.c_int
+    L.dpft_group_norm_workspace_size.argtypes = [P(GroupNorm)]
+    L.dpft_group_norm_workspace_size.restype = sz
+    L.dpft_group_norm_act.argtypes = [P(GroupNorm)] + [vp] * 9 + [sz, vp]
+    L.dpft_group_norm_act.restype = ctypes.c_int
+    L.dpft_group_norm_act_backward.argtypes = [P(GroupNorm)] + [vp] * 12 + [sz, vp]
+    L.dpft_group_norm_act_backward.restype = ctypes.c_int
+    L.dpft_act_checkpoint.argtypes = [vp, ctypes.c_int32, ctypes.c_int64, vp, vp, vp]
+    L.dpft_act_checkpoint.restype = ctypes.c_int
+    L.dpft_act_restore.argtypes = [vp, vp, ctypes.c_int64, vp, ctypes.c_int32, vp]
+    L.dpft_act_restore.restype = ctypes.c_int
     L.dpft_ic_damped_update.argtypes = [vp, vp, vp, ctypes.c_int32, ctypes.c_int32, vp, vp, vp, vp, vp]
     L.dpft_ic_damped_update.restype = ctypes.c_int
     i32 = ctypes.c_int32

@@ -54,6 +54,7 @@
 #include <vector>
 
 #include "dpft_ic.h"
+#include "dpft_internal.h"
 #include "dpft_tuning.h"
 
 // LLVM buffer-load intrinsics (declared at global scope: they bind by asm label).
@@ -4208,3 +4209,12 @@ int dpft_version(void) { return DPFT_ABI_VERSION; }
 const char* dpft_last_error(void) { return g_err; }
 
 }  // extern "C"
+
+int dpft_fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_err, sizeof(g_err), fmt, ap);
+  va_end(ap);
+  return code;
+}
+int dpft_hip_check(const char* what) { return hip_check(what); }

@@ -300,6 +300,70 @@ int dpft_bn_elu_pack(const float* x, const float* chan, float* out, int32_t B, i
                      void* hip_stream);
 
 /*
+ * Group normalisation with an activation, channels last: the epilogue of an encoder block
+ * (conv -> norm -> activation) whose statistics come from the sample itself, so that it is
+ * the same in training and in eval mode and does not depend on the batch.
+ *
+ * x [N][pixels][C] (channels_last storage, any C >= 1), `groups` divides C; per sample n and
+ * group g of D = C / groups channels, over pixels x D values:
+ *   mean = E[x], rstd = 1 / sqrt(E[(x - mean)^2] + eps),
+ *   z = (x - mean) * rstd * weight[c] + bias[c],  y = act(z).
+ * Values are fp32, bf16 or fp16 (x_type; y, dy and dx have x's); weight / bias (NULL: 1 / 0)
+ * and their gradients have param_type.  Statistics and sums are fp32, in a fixed order:
+ * bit-identical from run to run.  A non-finite value makes its (sample, group) NaN.
+ *
+ *  dpft_group_norm_act           mean_out / rstd_out [N][groups] fp32 (NULL: not wanted; the
+ *                                backward reads them).  q_out / scale_out (NULL: not wanted):
+ *                                x's 8-bit checkpoint, as dpft_act_checkpoint writes it.
+ *                                DPFT_GN_PACKED: y in the solver's channel-quad layout
+ *                                [N][C/4][pixels][4] (fp32, C % 4 == 0, no checkpoint).
+ *  dpft_group_norm_act_backward  dy -> dx, dweight, dbias [C] (each NULL: not wanted), from x
+ *                                or, with x NULL, from its checkpoint q / scale (x restored
+ *                                inside the kernels): with g = dy act'(z),
+ *                                dbias = sum g, dweight = sum g xhat and
+ *                                dx = rstd (weight g - E[weight g] - xhat E[weight g xhat]).
+ * The workspace needs no initialisation and holds nothing between calls; one call at a time
+ * may use it.  x / y / dy / dx are 16-byte aligned and not aliased.
+ */
+#define DPFT_TYPE_F32  0
+#define DPFT_TYPE_BF16 1
+#define DPFT_TYPE_F16  2
+#define DPFT_ACT_NONE 0
+#define DPFT_ACT_RELU 1
+#define DPFT_ACT_ELU  2 /* alpha = 1 */
+#define DPFT_ACT_SILU 3
+#define DPFT_GN_PACKED 0x1u
+typedef struct DpftGroupNorm {
+  int64_t pixels; /* H * W */
+  int32_t N, C, groups;
+  int32_t act;        /* DPFT_ACT_* */
+  int32_t x_type;     /* DPFT_TYPE_* */
+  int32_t param_type; /* DPFT_TYPE_* */
+  uint32_t flags;
+  float eps;
+} DpftGroupNorm;
+size_t dpft_group_norm_workspace_size(const DpftGroupNorm* desc); /* of either call; 0: bad descriptor */
+int dpft_group_norm_act(const DpftGroupNorm* desc, const void* x, const void* weight, const void* bias, void* y,
+                        float* mean_out, float* rstd_out, int8_t* q_out, uint8_t* scale_out, void* workspace,
+                        size_t workspace_bytes, void* hip_stream);
+int dpft_group_norm_act_backward(const DpftGroupNorm* desc, const void* dy, const void* x, const int8_t* q,
+                                 const uint8_t* scale, const void* weight, const void* bias, const float* mean,
+                                 const float* rstd, void* dx, void* dweight, void* dbias, void* workspace,
+                                 size_t workspace_bytes, void* hip_stream);
+
+/*
+ * Activation checkpoints in 8 bits: n values x (fp32, bf16 or fp16) in blocks of 32 in memory
+ * order, q [n] signed bytes and scale [(n + 31) / 32] bytes.  With E the biased fp32 exponent of
+ * the block's largest magnitude, clamped to [7, 254], a step is 2^(E - 133) and
+ * q = clamp(rint(x / step), -127, 127): the largest value takes 64 .. 127 steps, each value is off
+ * by at most half a step (one step where the clamp applies), and every q * step is exact in fp32
+ * and bf16.  scale holds E; 255 marks a block with a non-finite value, which restores as NaN.
+ * q and scale are 16-byte aligned.
+ */
+int dpft_act_checkpoint(const void* x, int32_t type, int64_t n, int8_t* q, uint8_t* scale, void* hip_stream);
+int dpft_act_restore(const int8_t* q, const uint8_t* scale, int64_t n, void* out, int32_t type, void* hip_stream);
+
+/*
  * Jacobian API, materialised -- the reference solver's methods that the fused solve
  * never needs (it keeps J in registers); kept for callers and tests that inspect J.
  *  dpft_feature_gradient    feature_gradient (algorithms.py:1844-1865): unit-normalised

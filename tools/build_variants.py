@@ -26,8 +26,9 @@ def one(spec):
         src, _, flags = flags[1:].partition(":")
     out = os.path.join(ROOT, "tools", "libs", f"libdpft_{name}.so")
     os.makedirs(os.path.dirname(out), exist_ok=True)
-    cmd = [B.HIPCC, f"--offload-arch={B.ARCH}", "-O3", "-std=c++17", "-shared", "-fPIC", f"-I{B.INC}", f"-I{os.path.dirname(B.SRC)}",
-           "-Rpass-analysis=kernel-resource-usage", *[f for f in flags.split(",") if f], "-o", out, src]
+    others = [os.path.join(B.CSRC, f + ".o") for f in B.SOURCES if f != os.path.basename(B.SRC)]  # from build()
+    cmd = [B.HIPCC, f"--offload-arch={B.ARCH}", "-shared", *B.CFLAGS, "-Wno-error", f"-I{B.INC}", f"-I{B.CSRC}",
+           *[f for f in flags.split(",") if f], "-o", out, src, *others]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode:
         sys.stderr.write(r.stderr)

@@ -22,8 +22,7 @@ def waves_per_simd(regs):
 
 
 def report(extra=()):
-    cmd = [B.HIPCC, f"--offload-arch={B.ARCH}", "-O3", "-std=c++17", "-c", f"-I{B.INC}",
-           "-Rpass-analysis=kernel-resource-usage", *extra, "-o", os.devnull, B.SRC]
+    cmd = [B.HIPCC, f"--offload-arch={B.ARCH}", *B.CFLAGS, "-c", f"-I{B.INC}", *extra, "-o", os.devnull, B.SRC]
     out = subprocess.run(cmd, capture_output=True, text=True, check=True).stderr
     rows, cur = [], None
     for line in out.splitlines():
