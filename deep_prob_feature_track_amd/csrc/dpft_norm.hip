@@ -108,24 +108,92 @@ __device__ __forceinline__ float per_step_of(int scale) {
   return scale == 255 ? 0.0f : __uint_as_float((uint32_t)(260 - scale) << 23);
 }
 
+// max over the 32 / V neighbouring lanes that hold a block (aligned groups of 4 or 8 lanes).
+template <int LANES>
+__device__ __forceinline__ uint32_t block_max(uint32_t m) {
+  static_assert(LANES == 4 || LANES == 8);
+  m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0xB1, 0xF, 0xF, true));  // quad_perm [1,0,3,2]
+  m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x4E, 0xF, 0xF, true));  // quad_perm [2,3,0,1]
+  if constexpr (LANES == 8) m = max(m, (uint32_t)__builtin_amdgcn_mov_dpp((int)m, 0x141, 0xF, 0xF, true));
+  return m;
+}
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <int V>
+struct Bytes;  // V signed bytes
+template <>
+struct Bytes<4> {
+  typedef uint32_t type;
+};
+template <>
+struct Bytes<8> {
+  typedef u32x2 type;
+};
+__device__ __forceinline__ uint32_t pack4(int a, int b, int c, int d) {
+  return (a & 255) | (b & 255) << 8 | (c & 255) << 16 | (uint32_t)d << 24;
+}
+// One thread's V values of a block that 32 / V neighbouring lanes share: their bytes, and the
+// block's scale (the largest magnitude's bits carry its exponent; NaN and infinity have 255).
+template <int V>
+__device__ __forceinline__ typename Bytes<V>::type quantise_vec(const float (&v)[V], int& scale) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+  scale = scale_of(__uint_as_float(block_max<kBlock8 / V>(m)));
+  const float ps = per_step_of(scale);
+  int q[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) q[j] = quantise(v[j], ps);
+  const uint32_t keep = scale == 255 ? 0u : ~0u;
+  if constexpr (V == 4) return pack4(q[0], q[1], q[2], q[3]) & keep;
+  else return u32x2{pack4(q[0], q[1], q[2], q[3]) & keep, pack4(q[4], q[5], q[6], q[7]) & keep};
+}
+template <int V>
+__device__ __forceinline__ void restore_vec(typename Bytes<V>::type b, float step, float (&v)[V]) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    uint32_t word;
+    if constexpr (V == 4) word = b;
+    else word = b[j / 4];
+    v[j] = (float)(int8_t)(word >> (8 * (j % 4))) * step;
+  }
+}
+
+// 16 bytes of x per thread and step, kUnroll steps in flight; the block's maximum by lane shifts.
+// Bound by HBM.
+constexpr int kUnroll = 4;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void act_checkpoint_kernel(const T* __restrict__ x, int64_t n,
                                                                   int8_t* __restrict__ q, uint8_t* __restrict__ scale) {
-  const int64_t step = (int64_t)gridDim.x * kThreads;
-  for (int64_t b = (int64_t)blockIdx.x * kThreads + threadIdx.x; b * kBlock8 < n; b += step) {
-    const int64_t i0 = b * kBlock8;
-    const int m = (int)min((int64_t)kBlock8, n - i0);
-    float top = 0.0f;
-    bool finite = true;
-    for (int i = 0; i < m; ++i) {
-      const float v = fabsf((float)x[i0 + i]);
-      finite = finite && v < __builtin_inff();
-      top = fmaxf(top, v);
+  constexpr int V = Vec<T>::V;
+  typedef typename Bytes<V>::type Q;
+  const int64_t chunk = (int64_t)kThreads * V, stride = (int64_t)gridDim.x * kUnroll * chunk;
+  for (int64_t c0 = (int64_t)blockIdx.x * kUnroll * chunk; c0 < n; c0 += stride) {
+    const int64_t i0 = c0 + threadIdx.x * V;
+    if (c0 + kUnroll * chunk <= n) {
+      float v[kUnroll][V];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) load_vec(x + i0 + u * chunk, v[u]);
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const int64_t i = i0 + u * chunk;
+        int sc;
+        *reinterpret_cast<Q*>(q + i) = quantise_vec<V>(v[u], sc);
+        if (i % kBlock8 == 0) scale[i / kBlock8] = (uint8_t)sc;
+      }
+    } else {
+      for (int u = 0; u < kUnroll; ++u) {  // every lane takes part in its block's maximum
+        const int64_t i = i0 + u * chunk;
+        float v[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = i + j < n ? (float)x[i + j] : 0.0f;
+        int sc;
+        const Q b = quantise_vec<V>(v, sc);
+        if (i % kBlock8 == 0 && i < n) scale[i / kBlock8] = (uint8_t)sc;
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (i + j < n) q[i + j] = reinterpret_cast<const int8_t*>(&b)[j];
+      }
     }
-    const int sc = finite ? scale_of(top) : 255;
-    scale[b] = (uint8_t)sc;
-    const float ps = per_step_of(sc);
-    for (int i = 0; i < m; ++i) q[i0 + i] = sc == 255 ? 0 : (int8_t)quantise((float)x[i0 + i], ps);
   }
 }
 
@@ -133,8 +201,31 @@ template <typename T>
 __global__ __launch_bounds__(kThreads) void act_restore_kernel(const int8_t* __restrict__ q,
                                                                const uint8_t* __restrict__ scale, int64_t n,
                                                                T* __restrict__ out) {
-  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads)
-    out[i] = (T)((float)q[i] * step_of(scale[i / kBlock8]));
+  constexpr int V = Vec<T>::V;
+  typedef typename Bytes<V>::type Q;
+  const int64_t chunk = (int64_t)kThreads * V, stride = (int64_t)gridDim.x * kUnroll * chunk;
+  for (int64_t c0 = (int64_t)blockIdx.x * kUnroll * chunk; c0 < n; c0 += stride) {
+    const int64_t i0 = c0 + threadIdx.x * V;
+    if (c0 + kUnroll * chunk <= n) {
+      Q b[kUnroll];
+      int sc[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        b[u] = *reinterpret_cast<const Q*>(q + i0 + u * chunk);
+        sc[u] = scale[(i0 + u * chunk) / kBlock8];
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        float v[V];
+        restore_vec<V>(b[u], step_of(sc[u]), v);
+        store_vec(out + i0 + u * chunk, v);
+      }
+    } else {
+      for (int u = 0; u < kUnroll; ++u)
+        for (int64_t i = i0 + u * chunk; i < min(i0 + u * chunk + V, n); ++i)
+          out[i] = (T)((float)q[i] * step_of(scale[i / kBlock8]));
+    }
+  }
 }
 
 // ------------------------------------------------------------------ the walk over a sample
@@ -148,6 +239,8 @@ struct Walk {
   int32_t W, tiles;  // slots of a tile (at most kThreads), tiles of a row
   int32_t RS;     // rows that a workgroup visits side by side
   int32_t parts;  // row ranges of a sample, one workgroup (per tile) each
+  int32_t in_block;   // a thread's V values lie in one checkpoint block
+  int32_t lanes_block;  // ... and the rows that a workgroup visits side by side are whole blocks
 };
 
 struct Place {
@@ -314,9 +407,12 @@ struct Affine {
 };
 
 // y = act((x - mean) a + bias), a = rstd * weight.
-template <typename T, int ACT, bool PACKED>
+// MODE: y as x is stored, in the channel-quad layout, or with x's checkpoint (w.lanes_block).
+enum { kPlain, kPacked, kCheckpoint };
+template <typename T, int ACT, int MODE>
 __global__ __launch_bounds__(kThreads) void gn_apply_kernel(const T* __restrict__ x, Walk w, Affine f,
-                                                            T* __restrict__ y) {
+                                                            T* __restrict__ y, int8_t* __restrict__ q,
+                                                            uint8_t* __restrict__ scale) {
   constexpr int V = Vec<T>::V;
   const Place p = place(w);
   if (!p.active) return;
@@ -335,9 +431,15 @@ __global__ __launch_bounds__(kThreads) void gn_apply_kernel(const T* __restrict_
   for (; r < rf; r += w.RS) {
     float v[V];
     load_vec(src + r * w.Cv, v);
+    if constexpr (MODE == kCheckpoint) {
+      const int64_t i = p.n * w.L + r * w.Cv + (int64_t)p.slot * V;
+      int sc;
+      *reinterpret_cast<typename Bytes<V>::type*>(q + i) = quantise_vec<V>(v, sc);
+      if (i % kBlock8 == 0) scale[i / kBlock8] = (uint8_t)sc;
+    }
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = act_fwd<ACT>(fmaf(v[j] - mu[j], a[j], b[j]));
-    if constexpr (PACKED) store_vec(y + p.n * w.L + (p.slot * w.rows + r) * V, v);
+    if constexpr (MODE == kPacked) store_vec(y + p.n * w.L + (p.slot * w.rows + r) * V, v);
     else store_vec(dst + r * w.Cv, v);
   }
   if (r == w.full && r < p.r1) {
@@ -355,14 +457,20 @@ struct Source {
   const T* x;
   const int8_t* q;
   const uint8_t* scale;
+  int in_block;
   __device__ __forceinline__ float one(int64_t i) const {
     if constexpr (Q8) return (float)q[i] * step_of(scale[i / kBlock8]);
     else return (float)x[i];
   }
   __device__ __forceinline__ void vec(int64_t i, float (&v)[Vec<T>::V]) const {
     if constexpr (Q8) {
+      constexpr int V = Vec<T>::V;
+      if (in_block) {
+        restore_vec<V>(*reinterpret_cast<const typename Bytes<V>::type*>(q + i), step_of(scale[i / kBlock8]), v);
+      } else {
 #pragma unroll
-      for (int j = 0; j < Vec<T>::V; ++j) v[j] = one(i + j);
+        for (int j = 0; j < V; ++j) v[j] = one(i + j);
+      }
     } else {
       load_vec(x + i, v);
     }
@@ -563,6 +671,10 @@ Walk make_walk(const DpftGroupNorm& d) {
   w.W = std::min(w.S, kThreads);
   w.tiles = (w.S + w.W - 1) / w.W;
   w.RS = kThreads / w.W;
+  const int whole = kBlock8 / std::gcd(w.Cv, kBlock8);  // rows that make whole checkpoint blocks
+  if (w.RS >= whole) w.RS -= w.RS % whole;
+  w.in_block = w.L % V == 0;
+  w.lanes_block = w.tiles == 1 && w.RS % whole == 0 && w.L % kBlock8 == 0;
   w.full = w.L / w.Cv;
   w.rows = (w.L + w.Cv - 1) / w.Cv;
   const int64_t step = (int64_t)kBatch * w.RS;
@@ -573,9 +685,10 @@ Walk make_walk(const DpftGroupNorm& d) {
 }
 
 constexpr int64_t kMaxValues = int64_t(1) << 48;
-// Workgroups for `threads` threads, at most 2^20 of them (a launch holds fewer than 2^32 threads).
-unsigned grid_for(int64_t threads) {
-  return (unsigned)std::min<int64_t>((threads + kThreads - 1) / kThreads, int64_t(1) << 20);
+// Workgroups of the flat kernels for n values, at most 2^20 (a launch holds fewer than 2^32 threads).
+unsigned grid_for(int type, int64_t n) {
+  const int64_t per = (int64_t)kThreads * kUnroll * (type == DPFT_TYPE_F32 ? 4 : 8);
+  return (unsigned)std::min<int64_t>((n + per - 1) / per, int64_t(1) << 20);
 }
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 size_t part_bytes(const DpftGroupNorm& d, const Walk& w) {
@@ -588,16 +701,21 @@ size_t need(const DpftGroupNorm& d, const Walk& w) {
 bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
 
 template <typename T, int ACT>
-void launch_forward(const DpftGroupNorm& d, const Walk& w, const void* x, const Affine& f, void* y, hipStream_t st) {
+void launch_forward(const DpftGroupNorm& d, const Walk& w, const void* x, const Affine& f, void* y, int8_t* q,
+                    uint8_t* scale, hipStream_t st) {
   const dim3 grid((unsigned)(d.N * w.parts * w.tiles)), block(kThreads);
   const T* xs = static_cast<const T*>(x);
+  T* ys = static_cast<T*>(y);
   if constexpr (sizeof(T) == 4) {
     if (d.flags & DPFT_GN_PACKED) {
-      hipLaunchKernelGGL((gn_apply_kernel<T, ACT, true>), grid, block, 0, st, xs, w, f, static_cast<T*>(y));
+      hipLaunchKernelGGL((gn_apply_kernel<T, ACT, kPacked>), grid, block, 0, st, xs, w, f, ys, nullptr, nullptr);
       return;
     }
   }
-  hipLaunchKernelGGL((gn_apply_kernel<T, ACT, false>), grid, block, 0, st, xs, w, f, static_cast<T*>(y));
+  if (q && w.lanes_block)
+    hipLaunchKernelGGL((gn_apply_kernel<T, ACT, kCheckpoint>), grid, block, 0, st, xs, w, f, ys, q, scale);
+  else
+    hipLaunchKernelGGL((gn_apply_kernel<T, ACT, kPlain>), grid, block, 0, st, xs, w, f, ys, nullptr, nullptr);
 }
 
 template <typename T, int ACT, bool Q8>
@@ -665,10 +783,11 @@ int dpft_group_norm_act(const DpftGroupNorm* desc, const void* x, const void* we
                        static_cast<const T*>(x), w, part);
     hipLaunchKernelGGL(gn_finish_stats_kernel, dim3((unsigned)(d.N * d.groups)), dim3(kThreads), 0, st, part, w, d.eps,
                        mean, rstd);
-    launch_forward<T, decltype(act)::value>(d, w, x, f, y, st);
+    launch_forward<T, decltype(act)::value>(d, w, x, f, y, q_out, scale_out, st);
   });
   if (const int rc = dpft_hip_check("gn_apply_kernel")) return rc;
-  return q_out ? dpft_act_checkpoint(x, d.x_type, d.N * w.L, q_out, scale_out, hip_stream) : DPFT_OK;
+  // blocks that cross a thread's values or a workgroup's rows: a pass of their own
+  return q_out && !w.lanes_block ? dpft_act_checkpoint(x, d.x_type, d.N * w.L, q_out, scale_out, hip_stream) : DPFT_OK;
 }
 
 int dpft_group_norm_act_backward(const DpftGroupNorm* desc, const void* dy, const void* x, const int8_t* q,
@@ -691,10 +810,10 @@ int dpft_group_norm_act_backward(const DpftGroupNorm* desc, const void* dy, cons
     using T = decltype(tag);
     constexpr int A = decltype(act)::value;
     if (x)
-      launch_backward<T, A, false>(d, w, dy, Source<T, false>{static_cast<const T*>(x), nullptr, nullptr}, f, dx,
+      launch_backward<T, A, false>(d, w, dy, Source<T, false>{static_cast<const T*>(x), nullptr, nullptr, 0}, f, dx,
                                    dweight, dbias, static_cast<char*>(ws), st);
     else
-      launch_backward<T, A, true>(d, w, dy, Source<T, true>{nullptr, q, scale}, f, dx, dweight, dbias,
+      launch_backward<T, A, true>(d, w, dy, Source<T, true>{nullptr, q, scale, w.in_block}, f, dx, dweight, dbias,
                                   static_cast<char*>(ws), st);
   });
   return dpft_hip_check("gn_grad_input_kernel");
@@ -706,7 +825,7 @@ int dpft_act_checkpoint(const void* x, int32_t type, int64_t n, int8_t* q, uint8
   if (n < 1 || n > kMaxValues) return dpft_fail(DPFT_E_INVALID, "bad size %lld", (long long)n);
   if (misaligned(x) || misaligned(q) || misaligned(scale))
     return dpft_fail(DPFT_E_INVALID, "x, q and scale must be 16-byte aligned");
-  const dim3 grid(grid_for((n + kBlock8 - 1) / kBlock8)), block(kThreads);
+  const dim3 grid(grid_for(type, n)), block(kThreads);
   dispatch(type, DPFT_ACT_NONE, [&](auto tag, auto) {
     using T = decltype(tag);
     hipLaunchKernelGGL(act_checkpoint_kernel<T>, grid, block, 0, static_cast<hipStream_t>(hip_stream),
@@ -721,7 +840,7 @@ int dpft_act_restore(const int8_t* q, const uint8_t* scale, int64_t n, void* out
   if (n < 1 || n > kMaxValues) return dpft_fail(DPFT_E_INVALID, "bad size %lld", (long long)n);
   if (misaligned(out) || misaligned(q) || misaligned(scale))
     return dpft_fail(DPFT_E_INVALID, "out, q and scale must be 16-byte aligned");
-  const dim3 grid(grid_for(n)), block(kThreads);
+  const dim3 grid(grid_for(type, n)), block(kThreads);
   dispatch(type, DPFT_ACT_NONE, [&](auto tag, auto) {
     using T = decltype(tag);
     hipLaunchKernelGGL(act_restore_kernel<T>, grid, block, 0, static_cast<hipStream_t>(hip_stream), q, scale, n,
