@@ -15,6 +15,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <numeric>
+#include <type_traits>
 
 #include "dpft_ic.h"
 #include "dpft_internal.h"
@@ -33,19 +34,49 @@ struct Vec {
   typedef T type __attribute__((ext_vector_type(V)));
 };
 
+// At a uniform base and a thread's 32-bit offset in values (the access's scalar-base form).
 template <typename T>
-__device__ __forceinline__ void load_vec(const T* p, float (&v)[Vec<T>::V]) {
-  const auto r = __builtin_bit_cast(typename Vec<T>::type, *reinterpret_cast<const u32x4_any*>(p));
+__device__ __forceinline__ T* at(T* base, uint32_t off) {
+  typedef std::conditional_t<std::is_const_v<T>, const char, char> Byte;
+  return reinterpret_cast<T*>(reinterpret_cast<Byte*>(base) + (size_t)(off * (uint32_t)sizeof(T)));
+}
+template <typename T>
+__device__ __forceinline__ u32x4 load_raw(const T* p) {
+  return *reinterpret_cast<const u32x4_any*>(p);
+}
+template <typename T>
+__device__ __forceinline__ void widen(u32x4 raw, float (&v)[Vec<T>::V]) {
+  const auto r = __builtin_bit_cast(typename Vec<T>::type, raw);
 #pragma unroll
   for (int j = 0; j < Vec<T>::V; ++j) v[j] = (float)r[j];
 }
-// Rounds to T to nearest even: the values' own type.
+template <typename T>
+__device__ __forceinline__ void load_vec(const T* p, float (&v)[Vec<T>::V]) {
+  widen<T>(load_raw(p), v);
+}
+// The first m of V values, zeros behind them.
+template <typename T>
+__device__ __forceinline__ u32x4 load_first(const T* p, int m) {
+  typename Vec<T>::type r = {};
+#pragma unroll
+  for (int j = 0; j < Vec<T>::V; ++j)
+    if (j < m) r[j] = p[j];
+  return __builtin_bit_cast(u32x4, r);
+}
+template <typename T>
+__device__ __forceinline__ void store_first(T* p, const float (&v)[Vec<T>::V], int m) {
+#pragma unroll
+  for (int j = 0; j < Vec<T>::V; ++j)
+    if (j < m) p[j] = (T)v[j];
+}
+// Rounds to T to nearest even: the values' own type.  Non-temporal: kept in L2, the results drive out
+// what the next pass reads (8 x 32 x 480 x 640 fp32: 205 -> 178 us).
 template <typename T>
 __device__ __forceinline__ void store_vec(T* p, const float (&v)[Vec<T>::V]) {
   typename Vec<T>::type r;
 #pragma unroll
   for (int j = 0; j < Vec<T>::V; ++j) r[j] = (T)v[j];
-  *reinterpret_cast<u32x4_any*>(p) = __builtin_bit_cast(u32x4, r);
+  __builtin_nontemporal_store(__builtin_bit_cast(u32x4, r), reinterpret_cast<u32x4_any*>(p));
 }
 
 __device__ __forceinline__ float load_param(const void* p, int type, int i, float none) {
@@ -61,22 +92,26 @@ __device__ __forceinline__ void store_param(void* p, int type, int i, float v) {
 }
 
 // ------------------------------------------------------------------ activations
-// expm1 on z <= 0: its Taylor polynomial to z^8 above -1/2 (the next term is 1.4e-8 of the value
-// there), exp(z) - 1 below (no cancellation beyond a factor 2.5).
+// expm1 on z <= 0: its Taylor polynomial to z^6 above -1/4 (the next term is 4.8e-8 of the value
+// there), exp(z) - 1 below (whose error of 1.2 x 2^-24 is at most 5.5 x 2^-24 of the value).
+template <typename T>
 __device__ __forceinline__ float expm1_neg(float z) {
-  float q = 1.0f / 40320;
-  q = fmaf(q, z, 1.0f / 5040);
-  q = fmaf(q, z, 1.0f / 720);
+  if constexpr (sizeof(T) < 4) {
+    // for a result of 16 bits: to z^3 above -1/16 (the next term is 2^-16.6 of the value there), and
+    // 2^-19.7 below: against half a step of 2^-9 (bf16) or 2^-12 (fp16)
+    return z > -0.0625f ? fmaf(z * z, fmaf(z, 1.0f / 6, 0.5f), z) : __expf(z) - 1.0f;
+  }
+  float q = 1.0f / 720;
   q = fmaf(q, z, 1.0f / 120);
   q = fmaf(q, z, 1.0f / 24);
   q = fmaf(q, z, 1.0f / 6);
   q = fmaf(q, z, 0.5f);
-  return z > -0.5f ? fmaf(z * z, q, z) : __expf(z) - 1.0f;
+  return z > -0.25f ? fmaf(z * z, q, z) : __expf(z) - 1.0f;
 }
-template <int ACT>
+template <int ACT, typename T>
 __device__ __forceinline__ float act_fwd(float z) {
   if constexpr (ACT == DPFT_ACT_RELU) return z < 0.0f ? 0.0f : z;
-  if constexpr (ACT == DPFT_ACT_ELU) return z > 0.0f ? z : expm1_neg(z);
+  if constexpr (ACT == DPFT_ACT_ELU) return z > 0.0f ? z : expm1_neg<T>(z);
   if constexpr (ACT == DPFT_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.0f + __expf(-z));
   return z;
 }
@@ -229,174 +264,243 @@ __global__ __launch_bounds__(kThreads) void act_restore_kernel(const int8_t* __r
 }
 
 // ------------------------------------------------------------------ the walk over a sample
+// A workgroup (n, part, tile) visits the blocks part, part + parts, ... of sample n: a block is `deep`
+// vectors a thread of RS rows side by side, so that the grid reads one stretch of memory at a time.
 struct Walk {
   int64_t L;      // values of a sample
   int64_t rows;   // rows of Cv values, the last one cut short where L % Cv != 0
   int64_t full;   // whole rows
-  int64_t rpp;    // rows of a part
-  int32_t C, D, G;
+  int32_t N, C, D, G;
   int32_t Cv, S;  // values and 16-byte slots of a row
   int32_t W, tiles;  // slots of a tile (at most kThreads), tiles of a row
   int32_t RS;     // rows that a workgroup visits side by side
-  int32_t parts;  // row ranges of a sample, one workgroup (per tile) each
-  int32_t in_block;   // a thread's V values lie in one checkpoint block
+  int32_t parts, blocks;  // workgroups (per tile) and blocks of a sample
+  int32_t in_block;     // a thread's V values lie in one checkpoint block
   int32_t lanes_block;  // ... and the rows that a workgroup visits side by side are whole blocks
 };
+
+// Vectors of a block, which a thread has in flight: of the statistics, of the apply pass, of the backward's two.
+constexpr int kDeep = 8, kDeepApply = 4, kDeepSums = 2, kDeepGrad = 2;
 
 struct Place {
   int n, part, tile, slot, rr;
   bool active;
-  int64_t r, r1;  // the thread's first row, the part's end
+  uint32_t off;     // the thread's first value in RS rows
+  int channel;      // of the thread's first value
+  __device__ __forceinline__ Place(const Walk& w, int V, int b) {
+    tile = b % w.tiles;
+    const int np = b / w.tiles;
+    n = np / w.parts;
+    part = np - n * w.parts;
+    const int t = threadIdx.x;
+    rr = t / w.W;
+    slot = tile * w.W + (t - rr * w.W);
+    active = rr < w.RS && slot < w.S;
+    if (!active) {
+      rr = 0;
+      slot = tile * w.W;
+    }
+    off = rr * w.Cv + slot * V;
+    channel = slot * V % w.C;
+  }
 };
-__device__ __forceinline__ Place place(const Walk& w) {
-  Place p;
-  const int b = blockIdx.x;
-  p.tile = b % w.tiles;
-  const int np = b / w.tiles;
-  p.n = np / w.parts;
-  p.part = np - p.n * w.parts;
-  const int t = threadIdx.x;
-  p.rr = t / w.W;
-  p.slot = p.tile * w.W + (t - p.rr * w.W);
-  p.active = p.rr < w.RS && p.slot < w.S;
-  p.r = p.part * w.rpp + p.rr;
-  p.r1 = min(w.rows, (int64_t)(p.part + 1) * w.rpp);
-  return p;
+// Of block b: vectors 0 .. whole - 1 of every thread are the sample's, of vector `whole` the first
+// `tail` values (0 where there is none: whole == deep), none behind it.
+struct Block {
+  int whole, tail;
+  int64_t at;  // the block's first value
+  __device__ __forceinline__ Block(const Walk& w, const Place& p, int b, int deep, int V) {
+    const int64_t r0 = (int64_t)b * deep * w.RS;
+    at = p.n * w.L + r0 * w.Cv;
+    whole = (int)min((w.full - r0) / w.RS, (int64_t)deep);
+    const int64_t r = r0 + (int64_t)whole * w.RS + p.rr;
+    tail = whole == deep ? 0 : r < w.full ? V : r == w.full ? tail_values(w, p.slot, V) : 0;
+  }
+  // Values of the cut row that fall to `slot`.
+  static __device__ __forceinline__ int tail_values(const Walk& w, int slot, int V) {
+    const int64_t left = w.L - w.full * w.Cv - (int64_t)slot * V;
+    return (int)max((int64_t)0, min(left, (int64_t)V));
+  }
+};
+
+// Threads that share a group's (or a position's) sum: a power of two, at most a wave.
+__device__ __forceinline__ int sharers(int things) {
+  int q = 64;
+  while (q > 1 && q * things > kThreads) q >>= 1;
+  return q;
 }
-// Values of the cut row that fall to `slot`.
-__device__ __forceinline__ int tail_values(const Walk& w, int slot, int V) {
-  const int64_t left = w.L - w.full * w.Cv - (int64_t)slot * V;
-  return (int)max((int64_t)0, min(left, (int64_t)V));
+template <typename F>
+__device__ __forceinline__ F lanes_sum(F v, int q) {
+  for (int o = q >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
+  return v;
+}
+// f(i) by Q lanes over the entries i of group g in shared memory that lie in a tile: an entry for each
+// `per` values of a tile's row, RS rows.  The lanes share the longer of rows and entries of a row.
+template <typename F>
+__device__ __forceinline__ void over_entries(const Walk& w, int tile, int V, int per, int g, int lane, int Q, F&& f) {
+  const int lo = tile * w.W * V, hi = min(lo + w.W * V, w.Cv), RE = w.W * V / per;
+#pragma unroll 1
+  for (int k = g * w.D; k < hi; k += w.C) {  // the row's copies of the group's channels
+    const int e0 = (max(k, lo) - lo) / per, e1 = (min(k + w.D, hi) - lo) / per;
+    if (w.RS >= e1 - e0) {
+#pragma unroll 1
+      for (int e = e0; e < e1; ++e)
+#pragma unroll 1
+        for (int r = lane; r < w.RS; r += Q) f(r * RE + e);
+    } else {
+#pragma unroll 1
+      for (int r = 0; r < w.RS; ++r)
+#pragma unroll 1
+        for (int e = e0 + lane; e < e1; e += Q) f(r * RE + e);
+    }
+  }
 }
 
 // ------------------------------------------------------------------ forward
-constexpr int kBatch = 8;  // rows whose mean and spread a thread takes at once
-
-// Per (sample, part, position of a row): count, mean and sum of squares about that mean of the
-// part's values.  Each thread takes the exact mean of kBatch values, then their squares about it,
-// and joins the batches by the parallel-variance rule: no cancellation, whatever the mean is.
+// Records [n][parts * tiles][G]: mean, sum of squares about it and count of the workgroup's values of a
+// group.  A thread takes the exact mean of kDeep values of a position, then their squares about it, and
+// joins the batches by the parallel-variance rule; the threads are joined in the same way: nothing
+// cancels, whatever the mean is.
 template <typename T>
-__global__ __launch_bounds__(kThreads) void gn_stats_kernel(const T* __restrict__ x, Walk w, float4* __restrict__ part) {
+__global__ __launch_bounds__(kThreads) void gn_stats_kernel(const T* __restrict__ x, Walk w, float4* __restrict__ rec) {
   constexpr int V = Vec<T>::V;
   __shared__ float s_mean[kThreads * V], s_m2[kThreads * V], s_cnt[kThreads * V];
-  const Place p = place(w);
+  const Place p(w, V, blockIdx.x);
+  const int step = w.RS * w.Cv;
   float mean[V] = {}, m2[V] = {};
-  int cnt = 0, tail = 0;
-  if (p.active) {
-    const T* base = x + p.n * w.L + (int64_t)p.slot * V;
-    int64_t r = p.r;
-    const int64_t rf = min(p.r1, w.full);
-    int k = 0;
-    for (; r + (kBatch - 1) * w.RS < rf; r += kBatch * w.RS, ++k) {
-      float v[kBatch][V];
+  int k = 0, cnt = 0, tail = 0;
+#pragma unroll 1
+  for (int b = p.part; b < w.blocks; b += w.parts) {
+    const Block blk(w, p, b, kDeep, V);
+    const T* src = x + blk.at;
+    if (blk.whole == kDeep) {
+      u32x4 raw[kDeep];
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) load_vec(base + (r + u * w.RS) * w.Cv, v[u]);
-      const float f = __builtin_amdgcn_rcpf((float)(k + 1));
+      for (int u = 0; u < kDeep; ++u, src += step) raw[u] = load_raw(at(src, p.off));
+      const float f = __builtin_amdgcn_rcpf((float)(k + 1)), c = (float)(k * kDeep) * f;
+      float s[V] = {}, q[V] = {};
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u) {
+        float v[V];
+        widen<T>(raw[u], v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) s[j] += v[j];
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[j] *= 1.0f / kDeep;
+#pragma unroll
+      for (int u = 0; u < kDeep; ++u) {
+        float v[V];
+        widen<T>(raw[u], v);
+#pragma unroll
+        for (int j = 0; j < V; ++j) q[j] = fmaf(v[j] - s[j], v[j] - s[j], q[j]);
+      }
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        float s = 0.0f, q = 0.0f;
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) s += v[u][j];
-        const float mu = s * (1.0f / kBatch);
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) q = fmaf(v[u][j] - mu, v[u][j] - mu, q);
-        const float d = mu - mean[j];
+        const float d = s[j] - mean[j];
         mean[j] = fmaf(d, f, mean[j]);
-        m2[j] += fmaf(d * d, (float)(k * kBatch) * f, q);
+        m2[j] += fmaf(d * d, c, q[j]);
       }
-    }
-    cnt = k * kBatch;
-    for (; r < rf; r += w.RS) {
+      ++k;
+    } else {  // the sample's last block
+      cnt = k * kDeep;
+      auto add = [&](const float(&v)[V], int m) {
+        const float f = 1.0f / (float)(cnt + 1);
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j < m) {
+            const float d = v[j] - mean[j];
+            mean[j] = fmaf(d, f, mean[j]);
+            m2[j] = fmaf(d, v[j] - mean[j], m2[j]);
+          }
+      };
+#pragma unroll 1
+      for (int u = 0; u < blk.whole; ++u, src += step) {
+        float v[V];
+        widen<T>(load_raw(at(src, p.off)), v);
+        add(v, V);
+        ++cnt;
+      }
+      tail = blk.tail;
       float v[V];
-      load_vec(base + r * w.Cv, v);
-      const float f = 1.0f / (float)++cnt;
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = v[j] - mean[j];
-        mean[j] = fmaf(d, f, mean[j]);
-        m2[j] = fmaf(d, v[j] - mean[j], m2[j]);
-      }
-    }
-    if (r == w.full && r < p.r1) {
-      tail = tail_values(w, p.slot, V);
-      const float f = 1.0f / (float)(cnt + 1);
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (j < tail) {
-          const float v = (float)base[r * w.Cv + j];
-          const float d = v - mean[j];
-          mean[j] = fmaf(d, f, mean[j]);
-          m2[j] = fmaf(d, v - mean[j], m2[j]);
-        }
+      widen<T>(load_first(at(src, p.off), tail), v);
+      add(v, tail);
     }
   }
+  if (cnt == 0) cnt = k * kDeep;
+  const bool merged = w.D % V == 0;  // a thread's V values are one group's: one entry
+  const float none = p.active ? 1.0f : 0.0f;
+  if (merged) {
+    float mu = 0.0f, sq = 0.0f;
+    const float n = (float)(cnt * V + tail);
 #pragma unroll
-  for (int j = 0; j < V; ++j) {
-    s_mean[threadIdx.x * V + j] = mean[j];
-    s_m2[threadIdx.x * V + j] = m2[j];
-    s_cnt[threadIdx.x * V + j] = (float)(cnt + (j < tail));
+    for (int j = 0; j < V; ++j) mu = fmaf((float)(cnt + (j < tail)), mean[j], mu);
+    mu = n > 0.0f ? mu / n : 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) sq += fmaf((float)(cnt + (j < tail)) * (mean[j] - mu), mean[j] - mu, m2[j]);
+    s_mean[threadIdx.x] = mu;
+    s_m2[threadIdx.x] = sq;
+    s_cnt[threadIdx.x] = n * none;
+  } else {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      s_mean[threadIdx.x * V + j] = mean[j];
+      s_m2[threadIdx.x * V + j] = m2[j];
+      s_cnt[threadIdx.x * V + j] = (float)(cnt + (j < tail)) * none;
+    }
   }
   __syncthreads();
-  const int PW = w.W * V;  // positions of a tile; thread (rr, slot)'s values are at rr * PW + slot * V
-  for (int i = threadIdx.x; i < PW; i += kThreads) {
-    const int pos = p.tile * PW + i;
-    if (pos >= w.Cv) break;
-    float c = 0.0f, s = 0.0f;
-    for (int a = 0; a < w.RS; ++a) {
-      c += s_cnt[a * PW + i];
-      s = fmaf(s_cnt[a * PW + i], s_mean[a * PW + i], s);
-    }
-    const float mu = c > 0.0f ? s / c : 0.0f;
-    float q = 0.0f;
-    for (int a = 0; a < w.RS; ++a) {
-      const float d = s_mean[a * PW + i] - mu;
-      q += fmaf(s_cnt[a * PW + i] * d, d, s_m2[a * PW + i]);
-    }
-    part[((int64_t)p.n * w.parts + p.part) * w.Cv + pos] = make_float4(mu, q, c, 0.0f);
+  const int Q = sharers(w.G), lane = threadIdx.x & (Q - 1), per = merged ? V : 1;
+  rec += ((int64_t)(p.n * w.parts + p.part) * w.tiles + p.tile) * w.G;
+#pragma unroll 1
+  for (int g = threadIdx.x / Q; g < w.G; g += kThreads / Q) {
+    float cn = 0.0f, cs = 0.0f, cq = 0.0f;
+    over_entries(w, p.tile, V, per, g, lane, Q, [&](int i) {
+      cn += s_cnt[i];
+      cs = fmaf(s_cnt[i], s_mean[i], cs);
+    });
+    cn = lanes_sum(cn, Q);
+    cs = lanes_sum(cs, Q);
+    const float mu = cn > 0.0f ? cs / cn : 0.0f;
+    over_entries(w, p.tile, V, per, g, lane, Q, [&](int i) {
+      cq += fmaf(s_cnt[i] * (s_mean[i] - mu), s_mean[i] - mu, s_cnt[i] > 0.0f ? s_m2[i] : 0.0f);
+    });
+    cq = lanes_sum(cq, Q);
+    if (lane == 0) rec[g] = make_float4(mu, cq, cn, 0.0f);
   }
 }
 
-__device__ __forceinline__ double block_sum(double v, double* s) {
-  for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) s[threadIdx.x >> 6] = v;
-  __syncthreads();
-  v = 0.0;
-  for (int i = 0; i < kThreads / 64; ++i) v += s[i];
-  return v;
+// Sample n's statistics of group g from its records, by Q lanes in a fixed order: in fp64, where the
+// sums of n, n mean and m2 + n mean^2 do for the spread.  All Q lanes return them.
+__device__ __forceinline__ float2 join_stats(const float4* rec, int R, int G, int n, int g, int lane, int Q, float eps) {
+  const float4* r = rec + (int64_t)n * R * G + g;
+  double cn = 0.0, cs = 0.0, cq = 0.0;
+#pragma unroll 4
+  for (int i = lane; i < R; i += Q) {
+    const float4 a = r[(int64_t)i * G];
+    const double m = a.x, c = a.z;
+    cn += c;
+    cs += c * m;
+    cq += a.y + c * m * m;
+  }
+  cn = lanes_sum(cn, Q);
+  cs = lanes_sum(cs, Q);
+  cq = lanes_sum(cq, Q);
+  const double mu = cs / cn, sq = cq - cs * mu;
+  return make_float2((float)mu, (float)(1.0 / sqrt((sq < 0.0 ? 0.0 : sq) / cn + (double)eps)));  // keeps a NaN
 }
 
-// One workgroup per (sample, group): the parts joined in fp64, in a fixed order.
-__global__ __launch_bounds__(kThreads) void gn_finish_stats_kernel(const float4* __restrict__ part, Walk w, float eps,
-                                                                   float* __restrict__ mean, float* __restrict__ rstd) {
-  __shared__ double s_red[kThreads / 64];
-  const int n = blockIdx.x / w.G, g = blockIdx.x - n * w.G;
-  const int KD = w.Cv / w.G;
-  const float4* src = part + (int64_t)n * w.parts * w.Cv;
-  const int64_t total = (int64_t)w.parts * KD;
-  auto at = [&](int64_t e) {
-    const int64_t pt = e / KD;
-    const int i = (int)(e - pt * KD), k = i / w.D;
-    return src[pt * w.Cv + k * w.C + g * w.D + (i - k * w.D)];
-  };
-  double c = 0.0, s = 0.0;
-  for (int64_t e = threadIdx.x; e < total; e += kThreads) {
-    const float4 a = at(e);
-    c += a.z;
-    s += (double)a.z * a.x;
-  }
-  c = block_sum(c, s_red);
-  const double mu = block_sum(s, s_red) / c;
-  double q = 0.0;
-  for (int64_t e = threadIdx.x; e < total; e += kThreads) {
-    const float4 a = at(e);
-    const double d = a.x - mu;
-    q += a.y + a.z * d * d;
-  }
-  q = block_sum(q, s_red);
-  if (threadIdx.x == 0) {
-    mean[blockIdx.x] = (float)mu;
-    rstd[blockIdx.x] = (float)(1.0 / sqrt(q / c + (double)eps));
+// Where a workgroup cannot join a sample's groups itself: a wave per (sample, group).
+__global__ __launch_bounds__(kThreads) void gn_finish_stats_kernel(const float4* __restrict__ rec, int R, int N, int G,
+                                                                   float eps, float* __restrict__ mean,
+                                                                   float* __restrict__ rstd) {
+  const int64_t i = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  if (i >= (int64_t)N * G) return;
+  const int n = (int)(i / G), g = (int)(i - (int64_t)n * G), lane = threadIdx.x & 63;
+  const float2 r = join_stats(rec, R, G, n, g, lane, 64, eps);
+  if (lane == 0) {
+    mean[i] = r.x;
+    rstd[i] = r.y;
   }
 }
 
@@ -408,45 +512,102 @@ struct Affine {
 
 // y = act((x - mean) a + bias), a = rstd * weight.
 // MODE: y as x is stored, in the channel-quad layout, or with x's checkpoint (w.lanes_block).
+// rec: the workgroup joins the statistics itself (kFold groups at most), its part 0 stores them.
+constexpr int kFold = 128;
 enum { kPlain, kPacked, kCheckpoint };
 template <typename T, int ACT, int MODE>
 __global__ __launch_bounds__(kThreads) void gn_apply_kernel(const T* __restrict__ x, Walk w, Affine f,
-                                                            T* __restrict__ y, int8_t* __restrict__ q,
-                                                            uint8_t* __restrict__ scale) {
+                                                            const float4* __restrict__ rec, int R, float eps,
+                                                            float* mean_out, float* rstd_out, T* __restrict__ y,
+                                                            int8_t* __restrict__ q, uint8_t* __restrict__ scale) {
   constexpr int V = Vec<T>::V;
-  const Place p = place(w);
-  if (!p.active) return;
-  float mu[V], a[V], b[V];
+  __shared__ float s_mu[kFold], s_rs[kFold];
+  const Place p(w, V, blockIdx.x);
+  const int step = w.RS * w.Cv;
+  // The blocks backwards: the statistics' pass has read the last ones last.  The next block's loads are
+  // issued as the vectors of this one are used, the first one's before the statistics are joined.
+  int b = w.blocks - 1 - p.part;
+  u32x4 raw[kDeepApply];
+  Block blk(w, p, b, kDeepApply, V);
+  auto load = [&](int u) { raw[u] = load_raw(at(x + blk.at + (int64_t)u * step, p.off)); };
+  if (blk.whole == kDeepApply) {
+#pragma unroll
+    for (int u = 0; u < kDeepApply; ++u) load(u);
+  }
+  if (rec) {
+    const int Q = sharers(w.G), lane = threadIdx.x & (Q - 1);
+#pragma unroll 1
+    for (int g = threadIdx.x / Q; g < w.G; g += kThreads / Q) {
+      const float2 r = join_stats(rec, R, w.G, p.n, g, lane, Q, eps);
+      if (lane == 0) {
+        s_mu[g] = r.x;
+        s_rs[g] = r.y;
+        if (mean_out && p.part == 0 && p.tile == 0) {
+          mean_out[p.n * w.G + g] = r.x;
+          rstd_out[p.n * w.G + g] = r.y;
+        }
+      }
+    }
+    __syncthreads();
+  }
+  float mu[V], a[V], bias[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int c = (p.slot * V + j) % w.C, g = p.n * w.G + c / w.D;
-    mu[j] = f.mean[g];
-    a[j] = f.rstd[g] * load_param(f.weight, f.type, c, 1.0f);
-    b[j] = load_param(f.bias, f.type, c, 0.0f);
+    const int c0 = p.channel + j, c = c0 < w.C ? c0 : c0 % w.C, g = c / w.D;
+    mu[j] = rec ? s_mu[g] : f.mean[p.n * w.G + g];
+    a[j] = (rec ? s_rs[g] : f.rstd[p.n * w.G + g]) * load_param(f.weight, f.type, c, 1.0f);
+    bias[j] = load_param(f.bias, f.type, c, 0.0f);
   }
-  const T* src = x + p.n * w.L + (int64_t)p.slot * V;
-  T* dst = y + p.n * w.L + (int64_t)p.slot * V;
-  int64_t r = p.r;
-  const int64_t rf = min(p.r1, w.full);
-  for (; r < rf; r += w.RS) {
+  // in the channel-quad layout a slot's rows follow one another
+  const int out_step = MODE == kPacked ? w.RS * V : step;
+  auto one = [&](const float(&x1)[V], int m, int64_t o, T* out) {
     float v[V];
-    load_vec(src + r * w.Cv, v);
-    if constexpr (MODE == kCheckpoint) {
-      const int64_t i = p.n * w.L + r * w.Cv + (int64_t)p.slot * V;
+    if constexpr (MODE == kCheckpoint) {  // rows come in whole blocks: m is V or 0, alike over a block
       int sc;
-      *reinterpret_cast<typename Bytes<V>::type*>(q + i) = quantise_vec<V>(v, sc);
-      if (i % kBlock8 == 0) scale[i / kBlock8] = (uint8_t)sc;
+      const auto bytes = quantise_vec<V>(x1, sc);
+      if (m == V && p.active) {
+        *reinterpret_cast<typename Bytes<V>::type*>(at(q + o, p.off)) = bytes;
+        if (p.off % kBlock8 == 0) *at(scale + o / kBlock8, p.off / kBlock8) = (uint8_t)sc;  // o % 32 == 0
+      }
     }
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = act_fwd<ACT>(fmaf(v[j] - mu[j], a[j], b[j]));
-    if constexpr (MODE == kPacked) store_vec(y + p.n * w.L + (p.slot * w.rows + r) * V, v);
-    else store_vec(dst + r * w.Cv, v);
-  }
-  if (r == w.full && r < p.r1) {
-    const int tail = tail_values(w, p.slot, V);
+    for (int j = 0; j < V; ++j) v[j] = act_fwd<ACT, T>(fmaf(x1[j] - mu[j], a[j], bias[j]));
+    if (!p.active) return;
+    if (m == V) store_vec(out, v);
+    else if (MODE != kPacked) store_first(out, v, m);
+  };
+#pragma unroll 1
+  while (b >= 0) {
+    const int64_t o = blk.at;
+    T* out;
+    if constexpr (MODE == kPacked) out = y + p.n * w.L + (p.slot * w.rows + (o - p.n * w.L) / w.Cv + p.rr) * V;
+    else out = at(y + o, p.off);
+    const int whole = blk.whole, tail = blk.tail;
+    b -= w.parts;
+    if (whole == kDeepApply) {
+      if (b >= 0) blk = Block(w, p, b, kDeepApply, V);  // a block before a whole one: whole
 #pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (j < tail) dst[r * w.Cv + j] = (T)act_fwd<ACT>(fmaf((float)src[r * w.Cv + j] - mu[j], a[j], b[j]));
+      for (int u = 0; u < kDeepApply; ++u, out += out_step) {
+        float v[V];
+        widen<T>(raw[u], v);
+        if (b >= 0) load(u);
+        one(v, V, o + (int64_t)u * step, out);
+      }
+    } else {
+      const T* src = x + o;
+#pragma unroll 1
+      for (int u = 0; u <= whole; ++u, src += step, out += out_step) {
+        const int m = u < whole ? V : tail;
+        float v[V];
+        widen<T>(load_first(at(src, p.off), m), v);
+        one(v, m, o + (int64_t)u * step, out);
+      }
+      if (b >= 0) {
+        blk = Block(w, p, b, kDeepApply, V);
+#pragma unroll
+        for (int u = 0; u < kDeepApply; ++u) load(u);
+      }
+    }
   }
 }
 
@@ -458,186 +619,304 @@ struct Source {
   const int8_t* q;
   const uint8_t* scale;
   int in_block;
-  __device__ __forceinline__ float one(int64_t i) const {
-    if constexpr (Q8) return (float)q[i] * step_of(scale[i / kBlock8]);
-    else return (float)x[i];
+};
+template <typename T, bool Q8>
+struct Held {  // V of them
+  u32x4 v;
+  __device__ __forceinline__ void load(const Source<T, Q8>& x, int64_t o, uint32_t off) { v = load_raw(at(x.x + o, off)); }
+  __device__ __forceinline__ void get(float (&out)[Vec<T>::V]) const { widen<T>(v, out); }
+};
+template <typename T>
+struct Held<T, true> {  // whole ones need Source::in_block
+  typename Bytes<Vec<T>::V>::type q;
+  int scale;
+  __device__ __forceinline__ void load(const Source<T, true>& x, int64_t o, uint32_t off) {
+    q = *reinterpret_cast<const typename Bytes<Vec<T>::V>::type*>(at(x.q + o, off));
+    scale = x.scale[(o + off) / kBlock8];
   }
-  __device__ __forceinline__ void vec(int64_t i, float (&v)[Vec<T>::V]) const {
-    if constexpr (Q8) {
-      constexpr int V = Vec<T>::V;
-      if (in_block) {
-        restore_vec<V>(*reinterpret_cast<const typename Bytes<V>::type*>(q + i), step_of(scale[i / kBlock8]), v);
-      } else {
+  __device__ __forceinline__ void get(float (&out)[Vec<T>::V]) const { restore_vec<Vec<T>::V>(q, step_of(scale), out); }
+};
+// The first m values one by one, zeros behind them.
+template <typename T, bool Q8>
+__device__ __forceinline__ void values(const Source<T, Q8>& x, int64_t i, int m, float (&v)[Vec<T>::V]) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) v[j] = one(i + j);
-      }
-    } else {
-      load_vec(x + i, v);
+  for (int j = 0; j < Vec<T>::V; ++j) {
+    v[j] = 0.0f;
+    if (j < m) {
+      if constexpr (Q8) v[j] = (float)x.q[i + j] * step_of(x.scale[(i + j) / kBlock8]);
+      else v[j] = (float)x.x[i + j];
     }
   }
-};
+}
 
-// Per (sample, part, position): sum g and sum g (x - mean), g = dy act'(z).
-template <typename T, int ACT, bool Q8>
-__global__ __launch_bounds__(kThreads) void gn_grad_sums_kernel(const T* __restrict__ dy, Source<T, Q8> x, Walk w,
-                                                                Affine f, float2* __restrict__ part) {
-  constexpr int V = Vec<T>::V;
-  __shared__ float s_1[kThreads * V], s_2[kThreads * V];
-  const Place p = place(w);
-  float s1[V] = {}, s2[V] = {};
-  if (p.active) {
-    float mu[V], a[V], b[V];
+template <int V>
+struct Coefs {
+  float mu[V], a[V], b[V];
+  __device__ __forceinline__ Coefs(const Walk& w, const Place& p, const Affine& f) {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
-      const int c = (p.slot * V + j) % w.C, g = p.n * w.G + c / w.D;
+      const int c0 = p.channel + j, c = c0 < w.C ? c0 : c0 % w.C, g = p.n * w.G + c / w.D;
       mu[j] = f.mean[g];
       a[j] = f.rstd[g] * load_param(f.weight, f.type, c, 1.0f);
       b[j] = load_param(f.bias, f.type, c, 0.0f);
     }
-    const int64_t base = p.n * w.L + (int64_t)p.slot * V;
-    int64_t r = p.r;
-    const int64_t rf = min(p.r1, w.full);
-    for (; r < rf; r += w.RS) {
-      float v[V], d[V];
-      x.vec(base + r * w.Cv, v);
-      load_vec(dy + base + r * w.Cv, d);
+  }
+};
+
+// With g = dy act'(z): per (sample, part, position of a row) sum g and sum g xhat, and per (sample,
+// part, tile, group) sum weight g and sum weight g xhat.
+template <typename T, int ACT, bool Q8>
+__global__ __launch_bounds__(kThreads) void gn_grad_sums_kernel(const T* __restrict__ dy, Source<T, Q8> x, Walk w,
+                                                                Affine f, float2* __restrict__ pos_out,
+                                                                float2* __restrict__ rec) {
+  constexpr int V = Vec<T>::V;
+  __shared__ float s_1[kThreads * V], s_2[kThreads * V];
+  const Place p(w, V, blockIdx.x);
+  const Coefs<V> k(w, p, f);
+  const int step = w.RS * w.Cv;
+  float s1[V] = {}, s2[V] = {};
+  auto add = [&](const float(&v)[V], const float(&d)[V], int m) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float xc = v[j] - mu[j], g = d[j] * act_slope<ACT>(fmaf(xc, a[j], b[j]));
-        s1[j] += g;
-        s2[j] = fmaf(g, xc, s2[j]);
-      }
+    for (int j = 0; j < V; ++j) {
+      const float xc = j < m ? v[j] - k.mu[j] : 0.0f, g = d[j] * act_slope<ACT>(fmaf(xc, k.a[j], k.b[j]));  // d is 0 behind m
+      s1[j] += g;
+      s2[j] = fmaf(g, xc, s2[j]);
     }
-    if (r == w.full && r < p.r1) {
-      const int tail = tail_values(w, p.slot, V);
+  };
+#pragma unroll 1
+  for (int b = p.part; b < w.blocks; b += w.parts) {
+    const Block blk(w, p, b, kDeepSums, V);
+    if (blk.whole == kDeepSums && (!Q8 || x.in_block)) {
+      u32x4 hd[kDeepSums];
+      Held<T, Q8> hx[kDeepSums];
 #pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (j < tail) {
-          const int64_t i = base + r * w.Cv + j;
-          const float xc = x.one(i) - mu[j], g = (float)dy[i] * act_slope<ACT>(fmaf(xc, a[j], b[j]));
-          s1[j] += g;
-          s2[j] = fmaf(g, xc, s2[j]);
-        }
+      for (int u = 0; u < kDeepSums; ++u) {
+        hx[u].load(x, blk.at + (int64_t)u * step, p.off);
+        hd[u] = load_raw(at(dy + blk.at + (int64_t)u * step, p.off));
+      }
+#pragma unroll
+      for (int u = 0; u < kDeepSums; ++u) {
+        float v[V], d[V];
+        hx[u].get(v);
+        widen<T>(hd[u], d);
+        add(v, d, V);
+      }
+    } else {
+#pragma unroll 1
+      for (int u = 0; u < kDeepSums && u <= blk.whole; ++u) {
+        const int m = u < blk.whole ? V : blk.tail;
+        const int64_t o = blk.at + (int64_t)u * step + p.off;
+        float v[V], d[V];
+        values(x, o, m, v);
+        widen<T>(load_first(dy + o, m), d);
+        add(v, d, m);
+      }
     }
   }
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    s_1[threadIdx.x * V + j] = s1[j];
-    s_2[threadIdx.x * V + j] = s2[j];
+    s_1[threadIdx.x * V + j] = p.active ? s1[j] : 0.0f;
+    s_2[threadIdx.x * V + j] = p.active ? s2[j] : 0.0f;
   }
   __syncthreads();
   const int PW = w.W * V;
-  for (int i = threadIdx.x; i < PW; i += kThreads) {
-    const int pos = p.tile * PW + i;
-    if (pos >= w.Cv) break;
-    float t1 = 0.0f, t2 = 0.0f;
-    for (int k = 0; k < w.RS; ++k) {
-      t1 += s_1[k * PW + i];
-      t2 += s_2[k * PW + i];
+  {
+    const int P = sharers(PW), pl = threadIdx.x & (P - 1);
+#pragma unroll 1
+    for (int i = threadIdx.x / P; i < PW; i += kThreads / P) {
+      float t1 = 0.0f, t2 = 0.0f;
+#pragma unroll 1
+      for (int r = pl; r < w.RS; r += P) {
+        t1 += s_1[r * PW + i];
+        t2 += s_2[r * PW + i];
+      }
+      t1 = lanes_sum(t1, P);
+      t2 = lanes_sum(t2, P);
+      const int pos = p.tile * PW + i;
+      if (pl == 0 && pos < w.Cv) {
+        const int c = pos % w.C;
+        t2 *= f.rstd[p.n * w.G + c / w.D];
+        pos_out[(int64_t)(p.n * w.parts + p.part) * w.Cv + pos] = make_float2(t1, t2);
+        const float wt = load_param(f.weight, f.type, c, 1.0f);
+        s_1[i] = wt * t1;  // row 0's place, which only these lanes have read
+        s_2[i] = wt * t2;
+      }
     }
-    part[((int64_t)p.n * w.parts + p.part) * w.Cv + pos] = make_float2(t1, t2);
+  }
+  __syncthreads();
+  const int Q = sharers(w.G), lane = threadIdx.x & (Q - 1);
+  rec += ((int64_t)(p.n * w.parts + p.part) * w.tiles + p.tile) * w.G;
+  const int lo = p.tile * PW, hi = min(lo + PW, w.Cv);
+#pragma unroll 1
+  for (int g = threadIdx.x / Q; g < w.G; g += kThreads / Q) {
+    float m1 = 0.0f, m2 = 0.0f;
+#pragma unroll 1
+    for (int c = g * w.D; c < hi; c += w.C)
+#pragma unroll 1
+      for (int i = max(c, lo) + lane; i < min(c + w.D, hi); i += Q) {
+        m1 += s_1[i - lo];
+        m2 += s_2[i - lo];
+      }
+    m1 = lanes_sum(m1, Q);
+    m2 = lanes_sum(m2, Q);
+    if (lane == 0) rec[g] = make_float2(m1, m2);
   }
 }
 
-// One workgroup per (sample, group): the parts' sums per channel, sums[n][c] = (sum g, sum g xhat),
-// and the group's means of weight g and weight g xhat.
-__global__ __launch_bounds__(kThreads) void gn_finish_grads_kernel(const float2* __restrict__ part, Walk w, Affine f,
-                                                                   float2* __restrict__ sums,
-                                                                   float2* __restrict__ means) {
-  __shared__ double s_red[kThreads / 64];
-  const int n = blockIdx.x / w.G, g = blockIdx.x - n * w.G;
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int K = w.Cv / w.C;
-  const float2* src = part + (int64_t)n * w.parts * w.Cv;
-  const float rs = f.rstd[blockIdx.x];
+// rstd E[weight g] and rstd^2 E[weight g xhat] of sample n's group g, by Q lanes as join_stats.
+__device__ __forceinline__ float2 join_grads(const float2* rec, int R, const Walk& w, const Affine& f, int n, int g,
+                                             int lane, int Q) {
+  const float2* r = rec + (int64_t)n * R * w.G + g;
   double m1 = 0.0, m2 = 0.0;
-  for (int d = wave; d < w.D; d += kThreads / 64) {
-    const int c = g * w.D + d;
-    double s1 = 0.0, s2 = 0.0;
-    for (int64_t e = lane; e < (int64_t)w.parts * K; e += 64) {
-      const float2 a = src[(e / K) * w.Cv + (int)(e % K) * w.C + c];
+#pragma unroll 4
+  for (int i = lane; i < R; i += Q) {
+    const float2 a = r[(int64_t)i * w.G];
+    m1 += a.x;
+    m2 += a.y;
+  }
+  const double rs = f.rstd[n * w.G + g], each = rs / (double)(w.L / w.G);
+  return make_float2((float)(each * lanes_sum(m1, Q)), (float)(each * rs * lanes_sum(m2, Q)));
+}
+__global__ __launch_bounds__(kThreads) void gn_finish_grads_kernel(const float2* __restrict__ rec, int R, Walk w,
+                                                                   Affine f, float2* __restrict__ means) {
+  const int64_t i = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
+  if (i >= (int64_t)w.N * w.G) return;
+  const int n = (int)(i / w.G), g = (int)(i - (int64_t)n * w.G), lane = threadIdx.x & 63;
+  const float2 r = join_grads(rec, R, w, f, n, g, lane, 64);
+  if (lane == 0) means[i] = r;
+}
+
+// dweight and dbias from `rows` rows of (sum g, sum g xhat) per channel: 8 channels a workgroup, the
+// rows dealt to 32 threads each and joined in a fixed order in fp64.
+constexpr int kGradCh = 8;
+__device__ __forceinline__ void param_grads(const float2* __restrict__ pos, int64_t rows, int C, int type, void* dweight,
+                                            void* dbias, int block) {
+  constexpr int R = kThreads / kGradCh;
+  __shared__ double s_1[R][kGradCh], s_2[R][kGradCh];
+  const int k = threadIdx.x % kGradCh, r = threadIdx.x / kGradCh, c = block * kGradCh + k;
+  double s1 = 0.0, s2 = 0.0;
+  if (c < C)
+#pragma unroll 4
+    for (int64_t i = r; i < rows; i += R) {
+      const float2 a = pos[i * C + c];
       s1 += a.x;
       s2 += a.y;
     }
-    for (int o = 32; o > 0; o >>= 1) {
-      s1 += __shfl_xor(s1, o);
-      s2 += __shfl_xor(s2, o);
+  s_1[r][k] = s1;
+  s_2[r][k] = s2;
+  __syncthreads();
+  if (r == 0 && c < C) {
+    s1 = s2 = 0.0;
+    for (int i = 0; i < R; ++i) {
+      s1 += s_1[i][k];
+      s2 += s_2[i][k];
     }
-    s2 *= rs;
-    if (lane == 0) {
-      sums[(int64_t)n * w.C + c] = make_float2((float)s1, (float)s2);
-      const double wt = load_param(f.weight, f.type, c, 1.0f);
-      m1 += wt * s1;
-      m2 += wt * s2;
-    }
+    if (dbias) store_param(dbias, type, c, (float)s1);
+    if (dweight) store_param(dweight, type, c, (float)s2);
   }
-  m1 = block_sum(m1, s_red);
-  m2 = block_sum(m2, s_red);
-  const double cnt = (double)w.L / w.G;
-  if (threadIdx.x == 0) means[blockIdx.x] = make_float2((float)(m1 / cnt), (float)(m2 / cnt));
 }
 
-__global__ __launch_bounds__(kThreads) void gn_param_grads_kernel(const float2* __restrict__ sums, int N, int C,
-                                                                  int type, void* dweight, void* dbias) {
-  const int c = blockIdx.x * kThreads + threadIdx.x;
-  if (c >= C) return;
-  double s1 = 0.0, s2 = 0.0;
-  for (int n = 0; n < N; ++n) {
-    const float2 a = sums[(int64_t)n * C + c];
-    s1 += a.x;
-    s2 += a.y;
-  }
-  if (dbias) store_param(dbias, type, c, (float)s1);
-  if (dweight) store_param(dweight, type, c, (float)s2);
-}
+struct Params {  // of the parameters' gradients: the first `blocks` workgroups compute them
+  const float2* pos;
+  int64_t rows;
+  void *dweight, *dbias;
+  int32_t blocks;
+};
 
 // dx = a g - rstd E[weight g] - (x - mean) rstd^2 E[weight g xhat], a = rstd * weight.
 template <typename T, int ACT, bool Q8>
 __global__ __launch_bounds__(kThreads) void gn_grad_input_kernel(const T* __restrict__ dy, Source<T, Q8> x, Walk w,
-                                                                 Affine f, const float2* __restrict__ means,
+                                                                 Affine f, Params pg, const float2* __restrict__ rec,
+                                                                 int R, const float2* __restrict__ means,
                                                                  T* __restrict__ dx) {
   constexpr int V = Vec<T>::V;
-  const Place p = place(w);
-  if (!p.active) return;
-  float mu[V], a[V], b[V], m1[V], m2[V];
+  __shared__ float s_m1[kFold], s_m2[kFold];
+  if ((int)blockIdx.x < pg.blocks) {
+    param_grads(pg.pos, pg.rows, w.C, f.type, pg.dweight, pg.dbias, blockIdx.x);
+    return;
+  }
+  const Place p(w, V, blockIdx.x - pg.blocks);
+  const int step = w.RS * w.Cv;
+  const bool vectors = !Q8 || x.in_block;
+  int b = w.blocks - 1 - p.part;  // backwards and ahead, as gn_apply_kernel
+  u32x4 hd[kDeepGrad];
+  Held<T, Q8> hx[kDeepGrad];
+  Block blk(w, p, b, kDeepGrad, V);
+  auto load = [&](int u) {
+    hx[u].load(x, blk.at + (int64_t)u * step, p.off);
+    hd[u] = load_raw(at(dy + blk.at + (int64_t)u * step, p.off));
+  };
+  if (vectors && blk.whole == kDeepGrad) {
+#pragma unroll
+    for (int u = 0; u < kDeepGrad; ++u) load(u);
+  }
+  if (rec) {
+    const int Q = sharers(w.G), lane = threadIdx.x & (Q - 1);
+#pragma unroll 1
+    for (int g = threadIdx.x / Q; g < w.G; g += kThreads / Q) {
+      const float2 r = join_grads(rec, R, w, f, p.n, g, lane, Q);
+      if (lane == 0) {
+        s_m1[g] = r.x;
+        s_m2[g] = r.y;
+      }
+    }
+    __syncthreads();
+  }
+  const Coefs<V> k(w, p, f);
+  float m1[V], m2[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int c = (p.slot * V + j) % w.C, g = p.n * w.G + c / w.D;
-    const float rs = f.rstd[g];
-    mu[j] = f.mean[g];
-    a[j] = rs * load_param(f.weight, f.type, c, 1.0f);
-    b[j] = load_param(f.bias, f.type, c, 0.0f);
-    m1[j] = rs * means[g].x;
-    m2[j] = rs * rs * means[g].y;
+    const int c0 = p.channel + j, g = (c0 < w.C ? c0 : c0 % w.C) / w.D;
+    m1[j] = rec ? s_m1[g] : means[p.n * w.G + g].x;
+    m2[j] = rec ? s_m2[g] : means[p.n * w.G + g].y;
   }
-  const int64_t base = p.n * w.L + (int64_t)p.slot * V;
-  int64_t r = p.r;
-  const int64_t rf = min(p.r1, w.full);
-  auto grad = [&](int j, float v, float d) {
-    const float xc = v - mu[j], g = d * act_slope<ACT>(fmaf(xc, a[j], b[j]));
-    return fmaf(-xc, m2[j], fmaf(a[j], g, -m1[j]));
+  auto grad = [&](float(&v)[V], const float(&d)[V]) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float xc = v[j] - k.mu[j], g = d[j] * act_slope<ACT>(fmaf(xc, k.a[j], k.b[j]));
+      v[j] = fmaf(-xc, m2[j], fmaf(k.a[j], g, -m1[j]));
+    }
   };
-  for (; r < rf; r += w.RS) {
-    float v[V], d[V];
-    x.vec(base + r * w.Cv, v);
-    load_vec(dy + base + r * w.Cv, d);
+#pragma unroll 1
+  while (b >= 0) {
+    const int64_t o = blk.at;
+    const int whole = blk.whole, tail = blk.tail;
+    b -= w.parts;
+    if (b >= 0) blk = Block(w, p, b, kDeepGrad, V);  // a block before another: whole
+    if (vectors && whole == kDeepGrad) {
+      T* out = dx + o;
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] = grad(j, v[j], d[j]);
-    store_vec(dx + base + r * w.Cv, v);
-  }
-  if (r == w.full && r < p.r1) {
-    const int tail = tail_values(w, p.slot, V);
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-      if (j < tail) {
-        const int64_t i = base + r * w.Cv + j;
-        dx[i] = (T)grad(j, x.one(i), (float)dy[i]);
+      for (int u = 0; u < kDeepGrad; ++u, out += step) {
+        float v[V], d[V];
+        hx[u].get(v);
+        widen<T>(hd[u], d);
+        if (b >= 0) load(u);
+        grad(v, d);
+        if (p.active) store_vec(at(out, p.off), v);
       }
+    } else {
+#pragma unroll 1
+      for (int u = 0; u < kDeepGrad && u <= whole; ++u) {
+        const int m = u < whole ? V : tail;
+        const int64_t i = o + (int64_t)u * step + p.off;
+        float v[V], d[V];
+        values(x, i, m, v);
+        widen<T>(load_first(dy + i, m), d);
+        grad(v, d);
+        if (p.active) store_first(dx + i, v, m);
+      }
+      if (vectors && b >= 0) {
+#pragma unroll
+        for (int u = 0; u < kDeepGrad; ++u) load(u);
+      }
+    }
   }
 }
 
 // ------------------------------------------------------------------ host side
-constexpr int kMaxParts = 256, kWorkgroups = 2048;
+// Workgroups of the statistics and of the gradients' sums, whose records the others join, and of those
+// that write.  (Statistics, 8 x 32 x 480 x 640 fp32 in all: 512 168 us, 1024 175, 2048 186.)
+constexpr int kStatsWorkgroups = 512, kSumsWorkgroups = 768, kApplyWorkgroups = 1024, kGradWorkgroups = 1024;
 
 int check(const DpftGroupNorm* d) {
   if (!d) return dpft_fail(DPFT_E_INVALID, "null descriptor");
@@ -659,9 +938,11 @@ int check(const DpftGroupNorm* d) {
   return DPFT_OK;
 }
 
-Walk make_walk(const DpftGroupNorm& d) {
+// deep: vectors that a thread visits in a block.
+Walk make_walk(const DpftGroupNorm& d, int deep, int workgroups) {
   Walk w{};
   const int V = d.x_type == DPFT_TYPE_F32 ? 4 : 8;
+  w.N = d.N;
   w.C = d.C;
   w.G = d.groups;
   w.D = d.C / d.groups;
@@ -677,10 +958,8 @@ Walk make_walk(const DpftGroupNorm& d) {
   w.lanes_block = w.tiles == 1 && w.RS % whole == 0 && w.L % kBlock8 == 0;
   w.full = w.L / w.Cv;
   w.rows = (w.L + w.Cv - 1) / w.Cv;
-  const int64_t step = (int64_t)kBatch * w.RS;
-  const int64_t want = std::max<int64_t>(1, std::min<int64_t>(kMaxParts, kWorkgroups / ((int64_t)d.N * w.tiles)));
-  w.rpp = ((w.rows + want - 1) / want + step - 1) / step * step;
-  w.parts = (int)((w.rows + w.rpp - 1) / w.rpp);
+  w.blocks = (int)((w.rows + (int64_t)deep * w.RS - 1) / ((int64_t)deep * w.RS));
+  w.parts = (int)std::min<int64_t>(w.blocks, std::max<int64_t>(1, workgroups / ((int64_t)d.N * w.tiles)));
   return w;
 }
 
@@ -691,48 +970,64 @@ unsigned grid_for(int type, int64_t n) {
   return (unsigned)std::min<int64_t>((n + per - 1) / per, int64_t(1) << 20);
 }
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-size_t part_bytes(const DpftGroupNorm& d, const Walk& w) {
-  return round256((size_t)d.N * w.parts * w.Cv * sizeof(float4));
+// The workspace: the forward's records, then statistics that nobody asked for; the backward's records,
+// positions and, for many groups, means.
+size_t record_bytes(const Walk& w, size_t one) { return round256((size_t)w.N * w.parts * w.tiles * w.G * one); }
+size_t position_bytes(const Walk& w) { return round256((size_t)w.N * w.parts * w.Cv * sizeof(float2)); }
+size_t group_bytes(const Walk& w) { return round256((size_t)w.N * w.G * sizeof(float2)); }
+size_t need(const DpftGroupNorm& d) {
+  const Walk f = make_walk(d, kDeep, kStatsWorkgroups), b = make_walk(d, kDeepSums, kSumsWorkgroups);
+  return std::max(record_bytes(f, sizeof(float4)) + group_bytes(f),
+                  record_bytes(b, sizeof(float2)) + position_bytes(b) + group_bytes(b));
 }
-size_t need(const DpftGroupNorm& d, const Walk& w) {
-  return part_bytes(d, w) + round256((size_t)d.N * d.C * sizeof(float2)) +
-         round256((size_t)d.N * d.groups * sizeof(float2));
-}
+// The workgroups of the last pass join a sample's records themselves where there are few of them.
+bool fold(const Walk& w) { return w.G <= kFold && (int64_t)w.parts * w.tiles * w.G <= 8192; }
+unsigned waves_grid(int64_t waves) { return (unsigned)((waves + kThreads / 64 - 1) / (kThreads / 64)); }
+unsigned walk_grid(const Walk& w) { return (unsigned)(w.N * w.parts * w.tiles); }
 bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
 
-template <typename T, int ACT>
-void launch_forward(const DpftGroupNorm& d, const Walk& w, const void* x, const Affine& f, void* y, int8_t* q,
-                    uint8_t* scale, hipStream_t st) {
-  const dim3 grid((unsigned)(d.N * w.parts * w.tiles)), block(kThreads);
-  const T* xs = static_cast<const T*>(x);
-  T* ys = static_cast<T*>(y);
-  if constexpr (sizeof(T) == 4) {
-    if (d.flags & DPFT_GN_PACKED) {
-      hipLaunchKernelGGL((gn_apply_kernel<T, ACT, kPacked>), grid, block, 0, st, xs, w, f, ys, nullptr, nullptr);
-      return;
-    }
+template <typename T, int ACT, int MODE>
+void launch_forward(const DpftGroupNorm& d, const T* x, Affine f, float* mean_out, float* rstd_out, T* y, int8_t* q,
+                    uint8_t* scale, void* ws, hipStream_t st) {
+  const Walk ws1 = make_walk(d, kDeep, kStatsWorkgroups), w = make_walk(d, kDeepApply, kApplyWorkgroups);
+  const int R = ws1.parts * ws1.tiles;
+  const dim3 block(kThreads);
+  float4* rec = static_cast<float4*>(ws);
+  hipLaunchKernelGGL(gn_stats_kernel<T>, dim3(walk_grid(ws1)), block, 0, st, x, ws1, rec);
+  if (!fold(ws1)) {
+    float* stats = reinterpret_cast<float*>(static_cast<char*>(ws) + record_bytes(ws1, sizeof(float4)));
+    if (!mean_out) mean_out = stats;
+    if (!rstd_out) rstd_out = stats + (size_t)d.N * d.groups;
+    f.mean = mean_out;
+    f.rstd = rstd_out;
+    hipLaunchKernelGGL(gn_finish_stats_kernel, dim3(waves_grid((int64_t)d.N * d.groups)), block, 0, st, rec, R, d.N, d.groups,
+                       d.eps, mean_out, rstd_out);
+    rec = nullptr;
   }
-  if (q && w.lanes_block)
-    hipLaunchKernelGGL((gn_apply_kernel<T, ACT, kCheckpoint>), grid, block, 0, st, xs, w, f, ys, q, scale);
-  else
-    hipLaunchKernelGGL((gn_apply_kernel<T, ACT, kPlain>), grid, block, 0, st, xs, w, f, ys, nullptr, nullptr);
+  hipLaunchKernelGGL((gn_apply_kernel<T, ACT, MODE>), dim3(walk_grid(w)), block, 0, st, x, w, f, rec, R, d.eps, mean_out,
+                     rstd_out, y, q, scale);
 }
 
 template <typename T, int ACT, bool Q8>
-void launch_backward(const DpftGroupNorm& d, const Walk& w, const void* dy, Source<T, Q8> x, const Affine& f, void* dx,
-                     void* dweight, void* dbias, char* ws, hipStream_t st) {
-  float2* part = reinterpret_cast<float2*>(ws);
-  float2* sums = reinterpret_cast<float2*>(ws + part_bytes(d, w));
-  float2* means = reinterpret_cast<float2*>(ws + part_bytes(d, w) + round256((size_t)d.N * d.C * sizeof(float2)));
-  const dim3 grid((unsigned)(d.N * w.parts * w.tiles)), block(kThreads);
-  const T* g = static_cast<const T*>(dy);
-  hipLaunchKernelGGL((gn_grad_sums_kernel<T, ACT, Q8>), grid, block, 0, st, g, x, w, f, part);
-  hipLaunchKernelGGL(gn_finish_grads_kernel, dim3((unsigned)(d.N * d.groups)), block, 0, st, part, w, f, sums, means);
-  if (dweight || dbias)
-    hipLaunchKernelGGL(gn_param_grads_kernel, dim3((unsigned)((d.C + kThreads - 1) / kThreads)), block, 0, st, sums,
-                       d.N, d.C, d.param_type, dweight, dbias);
-  if (dx)
-    hipLaunchKernelGGL((gn_grad_input_kernel<T, ACT, Q8>), grid, block, 0, st, g, x, w, f, means, static_cast<T*>(dx));
+void launch_backward(const DpftGroupNorm& d, const T* dy, Source<T, Q8> x, const Affine& f, T* dx, void* dweight,
+                     void* dbias, void* ws, hipStream_t st) {
+  const Walk ws1 = make_walk(d, kDeepSums, kSumsWorkgroups), w = make_walk(d, kDeepGrad, kGradWorkgroups);
+  const int R = ws1.parts * ws1.tiles;
+  const dim3 block(kThreads);
+  x.in_block = w.in_block;
+  float2* rec = static_cast<float2*>(ws);
+  float2* pos = reinterpret_cast<float2*>(static_cast<char*>(ws) + record_bytes(ws1, sizeof(float2)));
+  float2* means = reinterpret_cast<float2*>(reinterpret_cast<char*>(pos) + position_bytes(ws1));
+  hipLaunchKernelGGL((gn_grad_sums_kernel<T, ACT, Q8>), dim3(walk_grid(ws1)), block, 0, st, dy, x, ws1, f, pos, rec);
+  const Params pg{pos, (int64_t)d.N * ws1.parts * (w.Cv / w.C), dweight, dbias,
+                  dweight || dbias ? (w.C + kGradCh - 1) / kGradCh : 0};
+  if (dx && !fold(ws1)) {
+    hipLaunchKernelGGL(gn_finish_grads_kernel, dim3(waves_grid((int64_t)d.N * d.groups)), block, 0, st, rec, R, w, f, means);
+    rec = nullptr;
+  }
+  if (dx || pg.blocks)
+    hipLaunchKernelGGL((gn_grad_input_kernel<T, ACT, Q8>), dim3(pg.blocks + (dx ? walk_grid(w) : 0)), block, 0, st, dy, x,
+                       w, f, pg, rec, R, means, dx);
 }
 
 // f(type tag, activation constant) for the descriptor's value type and activation.
@@ -756,7 +1051,7 @@ extern "C" {
 
 size_t dpft_group_norm_workspace_size(const DpftGroupNorm* desc) {
   if (check(desc) != DPFT_OK) return 0;
-  return need(*desc, make_walk(*desc));
+  return need(*desc);
 }
 
 int dpft_group_norm_act(const DpftGroupNorm* desc, const void* x, const void* weight, const void* bias, void* y,
@@ -765,25 +1060,28 @@ int dpft_group_norm_act(const DpftGroupNorm* desc, const void* x, const void* we
   if (const int rc = check(desc)) return rc;
   const DpftGroupNorm& d = *desc;
   if (!x || !y || !ws || x == y) return dpft_fail(DPFT_E_INVALID, "null or aliased pointer");
+  if (!mean_out != !rstd_out) return dpft_fail(DPFT_E_INVALID, "the statistics need both mean_out and rstd_out");
   if (!q_out != !scale_out) return dpft_fail(DPFT_E_INVALID, "a checkpoint needs both q_out and scale_out");
   if (q_out && (d.flags & DPFT_GN_PACKED)) return dpft_fail(DPFT_E_INVALID, "no checkpoint with DPFT_GN_PACKED");
   if (misaligned(x) || misaligned(y) || misaligned(ws) || misaligned(q_out) || misaligned(scale_out))
     return dpft_fail(DPFT_E_INVALID, "x, y, the checkpoint and the workspace must be 16-byte aligned");
-  const Walk w = make_walk(d);
-  if (ws_bytes < need(d, w)) return dpft_fail(DPFT_E_WORKSPACE, "workspace %zu < %zu", ws_bytes, need(d, w));
+  const Walk w = make_walk(d, kDeepApply, kApplyWorkgroups);
+  if (ws_bytes < need(d)) return dpft_fail(DPFT_E_WORKSPACE, "workspace %zu < %zu", ws_bytes, need(d));
   hipStream_t st = static_cast<hipStream_t>(hip_stream);
-  float4* part = static_cast<float4*>(ws);
-  float* stats = reinterpret_cast<float*>(static_cast<char*>(ws) + part_bytes(d, w));
-  float* mean = mean_out ? mean_out : stats;
-  float* rstd = rstd_out ? rstd_out : stats + (size_t)d.N * d.groups;
-  const Affine f{weight, bias, mean, rstd, d.param_type};
+  const Affine f{weight, bias, nullptr, nullptr, d.param_type};
   dispatch(d.x_type, d.act, [&](auto tag, auto act) {
     using T = decltype(tag);
-    hipLaunchKernelGGL(gn_stats_kernel<T>, dim3((unsigned)(d.N * w.parts * w.tiles)), dim3(kThreads), 0, st,
-                       static_cast<const T*>(x), w, part);
-    hipLaunchKernelGGL(gn_finish_stats_kernel, dim3((unsigned)(d.N * d.groups)), dim3(kThreads), 0, st, part, w, d.eps,
-                       mean, rstd);
-    launch_forward<T, decltype(act)::value>(d, w, x, f, y, q_out, scale_out, st);
+    constexpr int A = decltype(act)::value;
+    const T* xs = static_cast<const T*>(x);
+    T* ys = static_cast<T*>(y);
+    if constexpr (sizeof(T) == 4) {
+      if (d.flags & DPFT_GN_PACKED)
+        return launch_forward<T, A, kPacked>(d, xs, f, mean_out, rstd_out, ys, nullptr, nullptr, ws, st);
+    }
+    if (q_out && w.lanes_block)
+      launch_forward<T, A, kCheckpoint>(d, xs, f, mean_out, rstd_out, ys, q_out, scale_out, ws, st);
+    else
+      launch_forward<T, A, kPlain>(d, xs, f, mean_out, rstd_out, ys, nullptr, nullptr, ws, st);
   });
   if (const int rc = dpft_hip_check("gn_apply_kernel")) return rc;
   // blocks that cross a thread's values or a workgroup's rows: a pass of their own
@@ -802,19 +1100,19 @@ int dpft_group_norm_act_backward(const DpftGroupNorm* desc, const void* dy, cons
   if (dx && (dx == dy || dx == x)) return dpft_fail(DPFT_E_INVALID, "aliased pointer");
   if (misaligned(dy) || misaligned(x) || misaligned(dx) || misaligned(q) || misaligned(scale) || misaligned(ws))
     return dpft_fail(DPFT_E_INVALID, "dy, x, dx, the checkpoint and the workspace must be 16-byte aligned");
-  const Walk w = make_walk(d);
-  if (ws_bytes < need(d, w)) return dpft_fail(DPFT_E_WORKSPACE, "workspace %zu < %zu", ws_bytes, need(d, w));
+  if (ws_bytes < need(d)) return dpft_fail(DPFT_E_WORKSPACE, "workspace %zu < %zu", ws_bytes, need(d));
   hipStream_t st = static_cast<hipStream_t>(hip_stream);
   const Affine f{weight, bias, mean, rstd, d.param_type};
   dispatch(d.x_type, d.act, [&](auto tag, auto act) {
     using T = decltype(tag);
     constexpr int A = decltype(act)::value;
+    const T* g = static_cast<const T*>(dy);
+    T* gx = static_cast<T*>(dx);
     if (x)
-      launch_backward<T, A, false>(d, w, dy, Source<T, false>{static_cast<const T*>(x), nullptr, nullptr, 0}, f, dx,
-                                   dweight, dbias, static_cast<char*>(ws), st);
+      launch_backward<T, A, false>(d, g, Source<T, false>{static_cast<const T*>(x), nullptr, nullptr, 0}, f, gx, dweight,
+                                   dbias, ws, st);
     else
-      launch_backward<T, A, true>(d, w, dy, Source<T, true>{nullptr, q, scale, w.in_block}, f, dx, dweight, dbias,
-                                  static_cast<char*>(ws), st);
+      launch_backward<T, A, true>(d, g, Source<T, true>{nullptr, q, scale, 0}, f, gx, dweight, dbias, ws, st);
   });
   return dpft_hip_check("gn_grad_input_kernel");
 }

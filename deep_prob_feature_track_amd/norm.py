@@ -11,13 +11,15 @@ current stream to the C ABI and never synchronise; every call has a workspace of
 on several streams, and captured graphs, share nothing.  CPU tensors raise: the modules of
 models/submodules.py take the torch path for them.
 """
+import contextlib
 import ctypes
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
-from .ic import _eager_only, _ptr, _stream
+from .ic import _eager_only
 
 BLOCK = 32  # values that share a step in a checkpoint
 
@@ -29,22 +31,7 @@ def _check_device(x, what):
         raise RuntimeError(f"{what} needs a device tensor; there is no CPU fallback")
 
 
-def _nhwc(x):
-    """x [N,C,H,W] stored channels_last and 16-byte aligned (a copy where it is not)."""
-    if not x.is_contiguous(memory_format=torch.channels_last):
-        x = x.contiguous(memory_format=torch.channels_last)
-    elif x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.channels_last)
-    return x
-
-
-def _empty_nhwc(x):
-    return torch.empty(x.shape, dtype=x.dtype, device=x.device, memory_format=torch.channels_last)
-
-
 def _check_param(p, name, x):
-    if p is None:
-        return
     if p.dim() != 1 or p.shape[0] != x.shape[1]:
         raise ValueError(f"{name} must hold one value per channel ({x.shape[1]}), got {tuple(p.shape)}")
     if p.dtype not in N.TYPES:
@@ -53,22 +40,49 @@ def _check_param(p, name, x):
         raise ValueError(f"{name} is on {p.device}, expected {x.device}")
 
 
-def _param(p):
-    return None if p is None else p.detach().contiguous()
+def _nhwc(x):
+    """x [N,C,H,W] stored channels_last and 16-byte aligned (a copy where it is not)."""
+    if not x.is_contiguous(memory_format=torch.channels_last):
+        x = x.contiguous(memory_format=torch.channels_last)
+    if x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.channels_last)
+    return x
 
 
-def _desc(x, groups, weight, bias, eps, act, packed=False):
-    B, C, H, W = x.shape
-    return N.GroupNorm(H * W, B, C, groups, N.ACTS[act], N.TYPES[x.dtype],
-                       N.TYPES[(weight if weight is not None else bias).dtype]
-                       if weight is not None or bias is not None else 0, N.GN_PACKED if packed else 0, eps)
+def _empty_nhwc(x):
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device, memory_format=torch.channels_last)
 
 
-def _workspace(desc, device):
-    nbytes = N.lib().dpft_group_norm_workspace_size(ctypes.byref(desc))
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _on(device):
+    """Launches go to the tensors' device, whichever is the current one."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+@functools.lru_cache(maxsize=4096)
+def _plan(shape, groups, act, x_type, param_type, flags, eps):
+    """(descriptor, its address, workspace bytes) of a call's sizes and types."""
+    B, C, H, W = shape
+    desc = N.GroupNorm(H * W, B, C, groups, N.ACTS[act], x_type, param_type, flags, eps)
+    ref = ctypes.byref(desc)
+    nbytes = N.lib().dpft_group_norm_workspace_size(ref)
     if nbytes == 0:
         N.check(-1, "dpft_group_norm_workspace_size")
-    return torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes
+    return desc, ref, nbytes
+
+
+def _call(x, groups, weight, bias, eps, act, flags=0):
+    """(descriptor's address, workspace bytes, workspace) for x's sizes; a workspace of the call's own."""
+    p = weight if weight is not None else bias
+    _, ref, nbytes = _plan(tuple(x.shape), groups, act, N.TYPES[x.dtype], 0 if p is None else N.TYPES[p.dtype], flags, eps)
+    return ref, nbytes, torch.empty(nbytes, dtype=torch.uint8, device=x.device)
 
 
 class ActCheckpoint:
@@ -113,7 +127,7 @@ def act_checkpoint(x):
     if n:
         if x.data_ptr() % 16:
             x = x.clone(memory_format=torch.preserve_format)
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             N.check(N.lib().dpft_act_checkpoint(_ptr(x), N.TYPES[x.dtype], n, _ptr(q), _ptr(scale), _stream(x.device)),
                     "dpft_act_checkpoint")
     return c
@@ -128,54 +142,51 @@ def act_restore(c, dtype=None):
         raise TypeError(f"act_restore: float32, bfloat16 or float16 (got {dtype})")
     out = torch.empty_strided(c.shape, c.stride, dtype=dtype, device=c.q.device)
     if out.numel():
-        with torch.cuda.device(out.device):
+        with _on(out.device):
             N.check(N.lib().dpft_act_restore(_ptr(c.q), _ptr(c.scale), c.q.numel(), _ptr(out), N.TYPES[dtype],
                                              _stream(out.device)), "dpft_act_restore")
     return out
 
 
 def _forward(x, groups, weight, bias, eps, act, packed, stats, checkpoint):
-    """-> y, mean, rstd, q, scale (None where not asked for); x channels_last."""
+    """-> y, statistics [2,N,groups], q, scale (None where not asked for); x channels_last."""
     B, C, H, W = x.shape
     if packed:
         y = torch.empty(B, C // 4, H, W, 4, dtype=x.dtype, device=x.device)
     else:
         y = _empty_nhwc(x)
-    mean = rstd = q = scale = None
-    if stats:
-        mean = torch.empty(B, groups, dtype=torch.float32, device=x.device)
-        rstd = torch.empty(B, groups, dtype=torch.float32, device=x.device)
-    if checkpoint:
-        q, scale = _checkpoint_buffers(x.numel(), x.device)
+    stat = torch.empty(2, B, groups, dtype=torch.float32, device=x.device) if stats else None
+    q, scale = _checkpoint_buffers(x.numel(), x.device) if checkpoint else (None, None)
     if x.numel():
-        with torch.cuda.device(x.device):
-            d = _desc(x, groups, weight, bias, eps, act, packed)
-            ws, nbytes = _workspace(d, x.device)
-            N.check(N.lib().dpft_group_norm_act(ctypes.byref(d), _ptr(x), _ptr(weight), _ptr(bias), _ptr(y), _ptr(mean),
-                                                _ptr(rstd), _ptr(q), _ptr(scale), _ptr(ws), nbytes, _stream(x.device)),
-                    "dpft_group_norm_act")
-    return y, mean, rstd, q, scale
+        with _on(x.device):
+            ref, nbytes, ws = _call(x, groups, weight, bias, eps, act, N.GN_PACKED if packed else 0)
+            mean = _ptr(stat)
+            rc = N.lib().dpft_group_norm_act(ref, x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean,
+                                             mean + 4 * B * groups if stats else None, _ptr(q), _ptr(scale),
+                                             ws.data_ptr(), nbytes, _stream(x.device))
+            if rc:
+                N.check(rc, "dpft_group_norm_act")
+    return y, stat, q, scale
 
 
 class _GroupNormAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, groups, eps, act, checkpoint):
         x = _nhwc(x)
-        w, b = _param(weight), _param(bias)
-        y, mean, rstd, q, scale = _forward(x, groups, w, b, eps, act, False, True, checkpoint)
-        ctx.args = (groups, eps, act, x.shape)
-        ctx.dtype = x.dtype
-        ctx.save_for_backward(None if checkpoint else x, q, scale, weight, bias, mean, rstd)
+        w = weight if weight is None else weight.contiguous()
+        b = bias if bias is None else bias.contiguous()
+        y, stat, q, scale = _forward(x, groups, w, b, eps, act, False, True, checkpoint)
+        ctx.args = (groups, eps, act)
+        ctx.save_for_backward(None if checkpoint else x, q, scale, w, b, stat)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x, q, scale, weight, bias, mean, rstd = ctx.saved_tensors
-        groups, eps, act, shape = ctx.args
+        x, q, scale, w, b, stat = ctx.saved_tensors
+        groups, eps, act = ctx.args
         need_x, need_w, need_b = ctx.needs_input_grad[:3]
         dy = _nhwc(dy)
-        w, b = _param(weight), _param(bias)
         dx = _empty_nhwc(dy) if need_x else None
         dw = torch.empty_like(w) if need_w else None
         db = torch.empty_like(b) if need_b else None
@@ -184,13 +195,15 @@ class _GroupNormAct(torch.autograd.Function):
                 if t is not None:
                     t.zero_()
         else:
-            with torch.cuda.device(dy.device):
-                d = _desc(dy, groups, w, b, eps, act)
-                ws, nbytes = _workspace(d, dy.device)
-                N.check(N.lib().dpft_group_norm_act_backward(
-                    ctypes.byref(d), _ptr(dy), _ptr(x), _ptr(q), _ptr(scale), _ptr(w), _ptr(b), _ptr(mean), _ptr(rstd),
-                    _ptr(dx), _ptr(dw), _ptr(db), _ptr(ws), nbytes, _stream(dy.device)),
-                    "dpft_group_norm_act_backward")
+            with _on(dy.device):
+                ref, nbytes, ws = _call(dy, groups, w, b, eps, act)
+                mean = stat.data_ptr()
+                rc = N.lib().dpft_group_norm_act_backward(
+                    ref, dy.data_ptr(), _ptr(x), _ptr(q), _ptr(scale), _ptr(w), _ptr(b), mean,
+                    mean + 4 * dy.shape[0] * groups, _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), nbytes,
+                    _stream(dy.device))
+                if rc:
+                    N.check(rc, "dpft_group_norm_act_backward")
         return dx, dw, db, None, None, None, None
 
 
@@ -209,26 +222,29 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="elu", packe
         raise ValueError(f"group_norm_act needs a map [N,C,H,W], got {tuple(x.shape)}")
     if act not in N.ACTS:
         raise ValueError(f"act must be one of {sorted(N.ACTS)} (got {act!r})")
-    if groups < 1 or x.shape[1] % groups or x.shape[1] == 0:
-        raise ValueError(f"groups={groups} does not divide C={x.shape[1]}")
+    C = x.shape[1]
+    if groups < 1 or C % groups or C == 0:
+        raise ValueError(f"groups={groups} does not divide C={C}")
     if not eps >= 0:
         raise ValueError(f"eps must not be negative (got {eps})")
-    for name, p in (("weight", weight), ("bias", bias)):
-        _check_param(p, name, x)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise TypeError(f"weight and bias must have one dtype (got {weight.dtype}, {bias.dtype})")
-    grad = torch.is_grad_enabled() and (x.requires_grad or any(p is not None and p.requires_grad
-                                                               for p in (weight, bias)))
+    if weight is not None:
+        _check_param(weight, "weight", x)
+    if bias is not None:
+        _check_param(bias, "bias", x)
+        if weight is not None and weight.dtype != bias.dtype:
+            raise TypeError(f"weight and bias must have one dtype (got {weight.dtype}, {bias.dtype})")
+    grad = torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                        or (bias is not None and bias.requires_grad))
     if packed:
         if grad:
             raise RuntimeError("packed=True is the solver's input at inference: it has no backward")
-        if x.dtype != torch.float32 or x.shape[1] % 4:
+        if x.dtype != torch.float32 or C % 4:
             raise ValueError(f"packed=True needs fp32 and C % 4 == 0, got {x.dtype} {tuple(x.shape)}")
     _check_device(x, "group_norm_act")
     if grad:
         return _GroupNormAct.apply(x, weight, bias, groups, eps, act, checkpoint)
-    x = _nhwc(x.detach())
-    return _forward(x, groups, _param(weight), _param(bias), eps, act, packed, False, False)[0]
+    return _forward(_nhwc(x), groups, weight if weight is None else weight.contiguous(),
+                    bias if bias is None else bias.contiguous(), eps, act, packed, False, False)[0]
 
 
 class _Conv2dCheckpoint(torch.autograd.Function):
