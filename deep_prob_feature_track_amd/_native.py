@@ -12,6 +12,7 @@ import torch  # (must be imported before the HIP library, see above)
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libdpft_ic.so")
+TORCH_LIB_PATH = os.path.join(_HERE, "libdpft_torch.so")
 
 ITER_FIRST, ITER_REVERSE, ITER_NO_UPDATE = 0x1, 0x2, 0x4
 REMOVE_TRU_SIGMA = 0x1
@@ -156,3 +157,12 @@ def check(rc, what):
     if rc != 0:
         msg = lib().dpft_last_error().decode(errors="replace")
         raise RuntimeError(f"{what} failed ({rc}): {msg}")
+
+
+def torch_ops():
+    """torch.ops.dpft with the operators of libdpft_torch.so; raises if it is unavailable."""
+    lib()
+    if not os.path.exists(TORCH_LIB_PATH):
+        raise RuntimeError(f"{TORCH_LIB_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
+    torch.ops.load_library(TORCH_LIB_PATH)
+    return torch.ops.dpft

@@ -1,4 +1,4 @@
-"""Build libdpft_ic.so in-tree for gfx950 (hipcc cross-compiles without a GPU).
+"""Build libdpft_ic.so and libdpft_torch.so in-tree for gfx950 (hipcc cross-compiles without a GPU).
 
 The compile also emits the compiler's per-kernel resource report
 (-Rpass-analysis=kernel-resource-usage); the build fails if a hot kernel lost its
@@ -17,6 +17,8 @@ ROOT = os.path.dirname(HERE)
 CSRC = os.path.join(HERE, "csrc")
 SRC = os.path.join(CSRC, "dpft_ic.hip")  # the solver
 SOURCES = ("dpft_ic.hip", "dpft_norm.hip")  # dpft_norm.hip: the encoder's normalisation
+TORCH_SRC = "dpft_torch.cpp"  # the torch operators over them (host code)
+TORCH_OUT = os.path.join(HERE, "libdpft_torch.so")
 HEADERS = ("dpft_internal.h", "dpft_tuning.h")
 OUT = os.path.join(HERE, "libdpft_ic.so")
 INC = os.path.join(ROOT, "include")
@@ -127,16 +129,31 @@ NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 SOURCE_FLAGS = {"dpft_ic.hip": [], "dpft_norm.hip": NO_PACKED_FP32}
 
 
+def torch_flags():
+    """(compile, link) flags of libdpft_torch.so."""
+    import torch
+    root = os.path.dirname(torch.__file__)
+    return (["-x", "c++", "-std=c++17", "-O2", "-fPIC", "-Wall", "-Werror", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             "-isystem", f"{root}/include", "-isystem", f"{root}/include/torch/csrc/api/include",
+             "-isystem", "/opt/rocm/include"],
+            ["-shared", f"-L{root}/lib", "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", f"-L{HERE}", "-l:libdpft_ic.so",
+             "-Wl,-rpath,$ORIGIN", "-Wl,--no-undefined"])
+
+
 def build(force=False, verbose=False):
-    deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS] + [os.path.join(INC, "dpft_ic.h"), __file__]
-    if not force and os.path.exists(OUT) and os.path.getmtime(OUT) >= max(os.path.getmtime(d) for d in deps):
+    deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS + (TORCH_SRC,)] + [os.path.join(INC, "dpft_ic.h"), __file__]
+    newest = max(os.path.getmtime(d) for d in deps)
+    if not force and all(os.path.exists(o) and os.path.getmtime(o) >= newest for o in (OUT, TORCH_OUT)):
         if not os.path.exists(ISA_OUT) or os.path.getmtime(ISA_OUT) < os.path.getmtime(OUT):
             write_isa_hashes()
         return OUT
+    cxx = os.path.join(LLVM_BIN, "clang++")
+    host_flags, link_flags = torch_flags()
+    cmds = [[HIPCC, f"--offload-arch={ARCH}", *CFLAGS, *SOURCE_FLAGS[f], f"-I{INC}"] for f in SOURCES] + [[cxx, *host_flags, f"-I{INC}"]]
     procs = []
-    for f in SOURCES:  # one compiler per source, side by side
+    for f, cmd in zip(SOURCES + (TORCH_SRC,), cmds):  # one compiler per source, side by side
         obj = os.path.join(CSRC, f + ".o")
-        cmd = [HIPCC, f"--offload-arch={ARCH}", *CFLAGS, *SOURCE_FLAGS[f], f"-I{INC}", "-c", "-o", obj, os.path.join(CSRC, f)]
+        cmd = cmd + ["-c", "-o", obj, os.path.join(CSRC, f)]
         if verbose:
             print(" ".join(cmd), file=sys.stderr)
         procs.append((cmd, obj, subprocess.Popen(cmd, stderr=subprocess.PIPE, text=True)))
@@ -146,9 +163,11 @@ def build(force=False, verbose=False):
             sys.stderr.write(err)
             raise subprocess.CalledProcessError(rc, cmd)
     check_occupancy(kernel_resources("".join(err for _, err, _ in results)))
-    subprocess.run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", OUT + ".tmp"] + [o for _, o, _ in procs],
-                   check=True)
+    objs = [o for _, o, _ in procs]
+    subprocess.run([HIPCC, f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", OUT + ".tmp"] + objs[:-1], check=True)
     os.replace(OUT + ".tmp", OUT)
+    subprocess.run([cxx, "-o", TORCH_OUT + ".tmp", objs[-1], *link_flags], check=True)
+    os.replace(TORCH_OUT + ".tmp", TORCH_OUT)
     write_isa_hashes()
     return OUT
 

@@ -6,14 +6,13 @@ from the sample itself: the same in training and in eval mode, at any batch size
 `conv2d` keeps its input that way for its weight gradient.  With `checkpoint=True` a block's
 backward pass needs 2 bytes a value of its two activations, not 8.
 
-Thin marshalling over libdpft_ic.so, as ic.py: they validate shapes, hand device pointers and the
-current stream to the C ABI and never synchronise; every call has a workspace of its own, so calls
-on several streams, and captured graphs, share nothing.  CPU tensors raise: the modules of
-models/submodules.py take the torch path for them.
+The operators are `torch.ops.dpft.*` of libdpft_torch.so over the C ABI (include/dpft_ic.h): they check
+their arguments, launch on the current stream of the tensors' device and never synchronise; every call
+has a workspace of its own, so that calls on several streams, and captured graphs, share nothing; they
+trace under torch.compile.  CPU tensors raise: the modules of models/submodules.py take the torch path
+for them.
 """
-import contextlib
-import ctypes
-import functools
+import os
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -23,66 +22,12 @@ from .ic import _eager_only
 
 BLOCK = 32  # values that share a step in a checkpoint
 
-
-def _check_device(x, what):
-    if x.dtype not in N.TYPES:
-        raise TypeError(f"{what}: float32, bfloat16 or float16 (got {x.dtype})")
-    if not x.is_cuda:
-        raise RuntimeError(f"{what} needs a device tensor; there is no CPU fallback")
+# loaded with the module, so that nothing is left to a traced call; without the library every call raises
+_ops = N.torch_ops() if os.path.exists(N.LIB_PATH) and os.path.exists(N.TORCH_LIB_PATH) else None
 
 
-def _check_param(p, name, x):
-    if p.dim() != 1 or p.shape[0] != x.shape[1]:
-        raise ValueError(f"{name} must hold one value per channel ({x.shape[1]}), got {tuple(p.shape)}")
-    if p.dtype not in N.TYPES:
-        raise TypeError(f"{name}: float32, bfloat16 or float16 (got {p.dtype})")
-    if p.device != x.device:
-        raise ValueError(f"{name} is on {p.device}, expected {x.device}")
-
-
-def _nhwc(x):
-    """x [N,C,H,W] stored channels_last and 16-byte aligned (a copy where it is not)."""
-    if not x.is_contiguous(memory_format=torch.channels_last):
-        x = x.contiguous(memory_format=torch.channels_last)
-    if x.data_ptr() % 16:
-        x = x.clone(memory_format=torch.channels_last)
-    return x
-
-
-def _empty_nhwc(x):
-    return torch.empty(x.shape, dtype=x.dtype, device=x.device, memory_format=torch.channels_last)
-
-
-def _ptr(t):
-    return None if t is None else t.data_ptr()
-
-
-def _on(device):
-    """Launches go to the tensors' device, whichever is the current one."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def _stream(device):
-    return torch._C._cuda_getCurrentRawStream(device.index)
-
-
-@functools.lru_cache(maxsize=4096)
-def _plan(shape, groups, act, x_type, param_type, flags, eps):
-    """(descriptor, its address, workspace bytes) of a call's sizes and types."""
-    B, C, H, W = shape
-    desc = N.GroupNorm(H * W, B, C, groups, N.ACTS[act], x_type, param_type, flags, eps)
-    ref = ctypes.byref(desc)
-    nbytes = N.lib().dpft_group_norm_workspace_size(ref)
-    if nbytes == 0:
-        N.check(-1, "dpft_group_norm_workspace_size")
-    return desc, ref, nbytes
-
-
-def _call(x, groups, weight, bias, eps, act, flags=0):
-    """(descriptor's address, workspace bytes, workspace) for x's sizes; a workspace of the call's own."""
-    p = weight if weight is not None else bias
-    _, ref, nbytes = _plan(tuple(x.shape), groups, act, N.TYPES[x.dtype], 0 if p is None else N.TYPES[p.dtype], flags, eps)
-    return ref, nbytes, torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+def _op(name):
+    return getattr(_ops if _ops is not None else N.torch_ops(), name).default
 
 
 class ActCheckpoint:
@@ -96,11 +41,6 @@ class ActCheckpoint:
 
     def nbytes(self):
         return self.q.numel() + self.scale.numel()
-
-
-def _checkpoint_buffers(n, device):
-    return (torch.empty(n, dtype=torch.int8, device=device),
-            torch.empty((n + BLOCK - 1) // BLOCK, dtype=torch.uint8, device=device))
 
 
 def _dense(x):
@@ -119,95 +59,18 @@ def act_checkpoint(x):
     memory order (a channels_last map: along its channels), each block with a step of 2^(E - 6) where
     2^E <= max |x| < 2^(E + 1): off by at most half a step, max |x| / 128 and less (a whole step where
     127 steps clamp the largest).  A block with an infinity or a NaN restores as NaN."""
-    _check_device(x, "act_checkpoint")
     x = _dense(x.detach())
-    n = x.numel()
-    q, scale = _checkpoint_buffers(n, x.device)
-    c = ActCheckpoint(q, scale, x.shape, x.stride(), x.dtype)
-    if n:
-        if x.data_ptr() % 16:
-            x = x.clone(memory_format=torch.preserve_format)
-        with _on(x.device):
-            N.check(N.lib().dpft_act_checkpoint(_ptr(x), N.TYPES[x.dtype], n, _ptr(q), _ptr(scale), _stream(x.device)),
-                    "dpft_act_checkpoint")
-    return c
+    q, scale = _op("act_checkpoint")(x)
+    return ActCheckpoint(q, scale, x.shape, x.stride(), x.dtype)
 
 
 @_eager_only
 def act_restore(c, dtype=None):
     """The values of an ActCheckpoint, in its own dtype or in `dtype` (exact in fp32 and bf16; rounded
     once in fp16 where its range ends)."""
-    dtype = c.dtype if dtype is None else dtype
-    if dtype not in N.TYPES:
-        raise TypeError(f"act_restore: float32, bfloat16 or float16 (got {dtype})")
-    out = torch.empty_strided(c.shape, c.stride, dtype=dtype, device=c.q.device)
-    if out.numel():
-        with _on(out.device):
-            N.check(N.lib().dpft_act_restore(_ptr(c.q), _ptr(c.scale), c.q.numel(), _ptr(out), N.TYPES[dtype],
-                                             _stream(out.device)), "dpft_act_restore")
-    return out
+    return _op("act_restore")(c.q, c.scale, c.shape, c.stride, c.dtype if dtype is None else dtype)
 
 
-def _forward(x, groups, weight, bias, eps, act, packed, stats, checkpoint):
-    """-> y, statistics [2,N,groups], q, scale (None where not asked for); x channels_last."""
-    B, C, H, W = x.shape
-    if packed:
-        y = torch.empty(B, C // 4, H, W, 4, dtype=x.dtype, device=x.device)
-    else:
-        y = _empty_nhwc(x)
-    stat = torch.empty(2, B, groups, dtype=torch.float32, device=x.device) if stats else None
-    q, scale = _checkpoint_buffers(x.numel(), x.device) if checkpoint else (None, None)
-    if x.numel():
-        with _on(x.device):
-            ref, nbytes, ws = _call(x, groups, weight, bias, eps, act, N.GN_PACKED if packed else 0)
-            mean = _ptr(stat)
-            rc = N.lib().dpft_group_norm_act(ref, x.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), mean,
-                                             mean + 4 * B * groups if stats else None, _ptr(q), _ptr(scale),
-                                             ws.data_ptr(), nbytes, _stream(x.device))
-            if rc:
-                N.check(rc, "dpft_group_norm_act")
-    return y, stat, q, scale
-
-
-class _GroupNormAct(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, groups, eps, act, checkpoint):
-        x = _nhwc(x)
-        w = weight if weight is None else weight.contiguous()
-        b = bias if bias is None else bias.contiguous()
-        y, stat, q, scale = _forward(x, groups, w, b, eps, act, False, True, checkpoint)
-        ctx.args = (groups, eps, act)
-        ctx.save_for_backward(None if checkpoint else x, q, scale, w, b, stat)
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, q, scale, w, b, stat = ctx.saved_tensors
-        groups, eps, act = ctx.args
-        need_x, need_w, need_b = ctx.needs_input_grad[:3]
-        dy = _nhwc(dy)
-        dx = _empty_nhwc(dy) if need_x else None
-        dw = torch.empty_like(w) if need_w else None
-        db = torch.empty_like(b) if need_b else None
-        if dy.numel() == 0:
-            for t in (dw, db):
-                if t is not None:
-                    t.zero_()
-        else:
-            with _on(dy.device):
-                ref, nbytes, ws = _call(dy, groups, w, b, eps, act)
-                mean = stat.data_ptr()
-                rc = N.lib().dpft_group_norm_act_backward(
-                    ref, dy.data_ptr(), _ptr(x), _ptr(q), _ptr(scale), _ptr(w), _ptr(b), mean,
-                    mean + 4 * dy.shape[0] * groups, _ptr(dx), _ptr(dw), _ptr(db), ws.data_ptr(), nbytes,
-                    _stream(dy.device))
-                if rc:
-                    N.check(rc, "dpft_group_norm_act_backward")
-        return dx, dw, db, None, None, None, None
-
-
-@_eager_only
 def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="elu", packed=False, checkpoint=False):
     """act(group_norm(x)) of a map [N,C,H,W] in fp32, bf16 or fp16, channels_last (other layouts are
     copied; the result is channels_last), differentiable once in x, weight and bias.
@@ -216,35 +79,12 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="elu", packe
     'none', 'relu', 'elu' or 'silu'.
     packed=True (inference, fp32, C % 4 == 0): the solver's channel-quad layout [N,C/4,H,W,4].
     checkpoint=True: the backward pass keeps x as an 8-bit checkpoint (act_checkpoint) instead of x,
-    written by the forward launch; y is that of x, the gradients are those at the restored x with x's
+    written by the forward pass; y is that of x, the gradients are those at the restored x with x's
     own statistics."""
-    if x.dim() != 4:
-        raise ValueError(f"group_norm_act needs a map [N,C,H,W], got {tuple(x.shape)}")
-    if act not in N.ACTS:
+    code = N.ACTS.get(act)
+    if code is None:
         raise ValueError(f"act must be one of {sorted(N.ACTS)} (got {act!r})")
-    C = x.shape[1]
-    if groups < 1 or C % groups or C == 0:
-        raise ValueError(f"groups={groups} does not divide C={C}")
-    if not eps >= 0:
-        raise ValueError(f"eps must not be negative (got {eps})")
-    if weight is not None:
-        _check_param(weight, "weight", x)
-    if bias is not None:
-        _check_param(bias, "bias", x)
-        if weight is not None and weight.dtype != bias.dtype:
-            raise TypeError(f"weight and bias must have one dtype (got {weight.dtype}, {bias.dtype})")
-    grad = torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
-                                        or (bias is not None and bias.requires_grad))
-    if packed:
-        if grad:
-            raise RuntimeError("packed=True is the solver's input at inference: it has no backward")
-        if x.dtype != torch.float32 or C % 4:
-            raise ValueError(f"packed=True needs fp32 and C % 4 == 0, got {x.dtype} {tuple(x.shape)}")
-    _check_device(x, "group_norm_act")
-    if grad:
-        return _GroupNormAct.apply(x, weight, bias, groups, eps, act, checkpoint)
-    return _forward(_nhwc(x), groups, weight if weight is None else weight.contiguous(),
-                    bias if bias is None else bias.contiguous(), eps, act, packed, False, False)[0]
+    return _op("group_norm_act")(x, groups, weight, bias, eps, code, packed, checkpoint)
 
 
 class _Conv2dCheckpoint(torch.autograd.Function):
@@ -278,7 +118,8 @@ def conv2d(x, weight, bias=None, stride=1, padding=0, dilation=1, groups=1):
     gradient of x, the weight's gradient at the restored x.  Under autocast, in its dtype."""
     if isinstance(padding, str):
         raise ValueError(f"padding must be numbers (got {padding!r})")
-    _check_device(x, "conv2d")
+    if not x.is_cuda:
+        raise RuntimeError("conv2d needs a device tensor; there is no CPU fallback")
     args = (_pair(stride), _pair(padding), _pair(dilation), groups)
     if not (torch.is_grad_enabled() and weight.requires_grad):  # the backward pass does not read x
         return torch.nn.functional.conv2d(x, weight, bias, *args)
