@@ -324,9 +324,9 @@ struct Block {
 };
 
 // Threads that share a group's (or a position's) sum: a power of two, at most a wave.
-__device__ __forceinline__ int sharers(int things) {
+__device__ __forceinline__ int sharers(int things, int threads = kThreads) {
   int q = 64;
-  while (q > 1 && q * things > kThreads) q >>= 1;
+  while (q > 1 && q * things > threads) q >>= 1;
   return q;
 }
 template <typename F>
@@ -368,66 +368,68 @@ __global__ __launch_bounds__(kThreads) void gn_stats_kernel(const T* __restrict_
   const Place p(w, V, blockIdx.x);
   const int step = w.RS * w.Cv;
   float mean[V] = {}, m2[V] = {};
-  int k = 0, cnt = 0, tail = 0;
+  int cnt = 0, tail = 0;
+  // The exact means of the first n vectors, their squares about them, and both joined to what there is.
+  // (Selects where n < kDeep: branches cost registers, and a branch a vector a fifth of the rate.)
+  auto join = [&](const u32x4(&raw)[kDeep], int n, auto whole) {
+    float s[V] = {}, q[V] = {};
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      float v[V];
+      widen<T>(raw[u], v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[j] += whole || u < n ? v[j] : 0.0f;
+    }
+    const float r = whole ? 1.0f / kDeep : 1.0f / (float)n;
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[j] *= r;
+#pragma unroll
+    for (int u = 0; u < kDeep; ++u) {
+      float v[V];
+      widen<T>(raw[u], v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = whole || u < n ? v[j] - s[j] : 0.0f;
+        q[j] = fmaf(d, d, q[j]);
+      }
+    }
+    const float f = (float)n * __builtin_amdgcn_rcpf((float)(cnt + n)), c = (float)cnt * f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float d = s[j] - mean[j];
+      mean[j] = fmaf(d, f, mean[j]);
+      m2[j] += fmaf(d * d, c, q[j]);
+    }
+    cnt += n;
+  };
 #pragma unroll 1
   for (int b = p.part; b < w.blocks; b += w.parts) {
     const Block blk(w, p, b, kDeep, V);
     const T* src = x + blk.at;
+    u32x4 raw[kDeep];
     if (blk.whole == kDeep) {
-      u32x4 raw[kDeep];
 #pragma unroll
-      for (int u = 0; u < kDeep; ++u, src += step) raw[u] = load_raw(at(src, p.off));
-      const float f = __builtin_amdgcn_rcpf((float)(k + 1)), c = (float)(k * kDeep) * f;
-      float s[V] = {}, q[V] = {};
-#pragma unroll
-      for (int u = 0; u < kDeep; ++u) {
-        float v[V];
-        widen<T>(raw[u], v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) s[j] += v[j];
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) s[j] *= 1.0f / kDeep;
-#pragma unroll
-      for (int u = 0; u < kDeep; ++u) {
-        float v[V];
-        widen<T>(raw[u], v);
-#pragma unroll
-        for (int j = 0; j < V; ++j) q[j] = fmaf(v[j] - s[j], v[j] - s[j], q[j]);
-      }
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        const float d = s[j] - mean[j];
-        mean[j] = fmaf(d, f, mean[j]);
-        m2[j] += fmaf(d * d, c, q[j]);
-      }
-      ++k;
+      for (int u = 0; u < kDeep; ++u) raw[u] = load_raw(at(src + (int64_t)u * step, p.off));
+      join(raw, kDeep, std::true_type{});
     } else {  // the sample's last block
-      cnt = k * kDeep;
-      auto add = [&](const float(&v)[V], int m) {
-        const float f = 1.0f / (float)(cnt + 1);
+      if (blk.whole) {
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (j < m) {
-            const float d = v[j] - mean[j];
-            mean[j] = fmaf(d, f, mean[j]);
-            m2[j] = fmaf(d, v[j] - mean[j], m2[j]);
-          }
-      };
-#pragma unroll 1
-      for (int u = 0; u < blk.whole; ++u, src += step) {
-        float v[V];
-        widen<T>(load_raw(at(src, p.off)), v);
-        add(v, V);
-        ++cnt;
+        for (int u = 0; u < kDeep; ++u) raw[u] = load_raw(at(src + (int64_t)min(u, blk.whole - 1) * step, p.off));
+        join(raw, blk.whole, std::false_type{});
       }
       tail = blk.tail;
       float v[V];
-      widen<T>(load_first(at(src, p.off), tail), v);
-      add(v, tail);
+      widen<T>(load_first(at(src + (int64_t)blk.whole * step, p.off), tail), v);
+      const float f = 1.0f / (float)(cnt + 1);
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j < tail) {
+          const float d = v[j] - mean[j];
+          mean[j] = fmaf(d, f, mean[j]);
+          m2[j] = fmaf(d, v[j] - mean[j], m2[j]);
+        }
     }
   }
-  if (cnt == 0) cnt = k * kDeep;
   const bool merged = w.D % V == 0;  // a thread's V values are one group's: one entry
   const float none = p.active ? 1.0f : 0.0f;
   if (merged) {
@@ -527,13 +529,13 @@ __global__ __launch_bounds__(kThreads) void gn_apply_kernel(const T* __restrict_
   // The blocks backwards: the statistics' pass has read the last ones last.  The next block's loads are
   // issued as the vectors of this one are used, the first one's before the statistics are joined.
   int b = w.blocks - 1 - p.part;
-  u32x4 raw[kDeepApply];
+  u32x4 raw[kDeepApply], end{};
   Block blk(w, p, b, kDeepApply, V);
   auto load = [&](int u) { raw[u] = load_raw(at(x + blk.at + (int64_t)u * step, p.off)); };
-  if (blk.whole == kDeepApply) {
 #pragma unroll
-    for (int u = 0; u < kDeepApply; ++u) load(u);
-  }
+  for (int u = 0; u < kDeepApply; ++u)
+    if (u < blk.whole) load(u);
+  if (blk.whole < kDeepApply) end = load_first(at(x + blk.at + (int64_t)blk.whole * step, p.off), blk.tail);
   if (rec) {
     const int Q = sharers(w.G), lane = threadIdx.x & (Q - 1);
 #pragma unroll 1
@@ -576,39 +578,187 @@ __global__ __launch_bounds__(kThreads) void gn_apply_kernel(const T* __restrict_
     if (m == V) store_vec(out, v);
     else if (MODE != kPacked) store_first(out, v, m);
   };
-#pragma unroll 1
-  while (b >= 0) {
+  auto first_out = [&](int64_t o) {
+    if constexpr (MODE == kPacked) return y + p.n * w.L + (p.slot * w.rows + (o - p.n * w.L) / w.Cv + p.rr) * V;
+    else return at(y + o, p.off);
+  };
+  if (blk.whole < kDeepApply) {  // the sample's last block
     const int64_t o = blk.at;
-    T* out;
-    if constexpr (MODE == kPacked) out = y + p.n * w.L + (p.slot * w.rows + (o - p.n * w.L) / w.Cv + p.rr) * V;
-    else out = at(y + o, p.off);
-    const int whole = blk.whole, tail = blk.tail;
-    b -= w.parts;
-    if (whole == kDeepApply) {
-      if (b >= 0) blk = Block(w, p, b, kDeepApply, V);  // a block before a whole one: whole
+    const int whole = blk.whole;
+    T* out = first_out(o);
+    float v[V];
 #pragma unroll
-      for (int u = 0; u < kDeepApply; ++u, out += out_step) {
-        float v[V];
+    for (int u = 0; u < kDeepApply - 1; ++u)
+      if (u < whole) {
         widen<T>(raw[u], v);
-        if (b >= 0) load(u);
-        one(v, V, o + (int64_t)u * step, out);
+        one(v, V, o + (int64_t)u * step, out + (int64_t)u * out_step);
       }
-    } else {
-      const T* src = x + o;
-#pragma unroll 1
-      for (int u = 0; u <= whole; ++u, src += step, out += out_step) {
-        const int m = u < whole ? V : tail;
-        float v[V];
-        widen<T>(load_first(at(src, p.off), m), v);
-        one(v, m, o + (int64_t)u * step, out);
-      }
-      if (b >= 0) {
-        blk = Block(w, p, b, kDeepApply, V);
+    widen<T>(end, v);
+    one(v, blk.tail, o + (int64_t)whole * step, out + (int64_t)whole * out_step);
+    b -= w.parts;
+    if (b < 0) return;
+    blk = Block(w, p, b, kDeepApply, V);
 #pragma unroll
-        for (int u = 0; u < kDeepApply; ++u) load(u);
+    for (int u = 0; u < kDeepApply; ++u) load(u);
+  }
+#pragma unroll 1
+  for (;;) {
+    const int64_t o = blk.at;
+    T* out = first_out(o);
+    b -= w.parts;
+    const bool more = b >= 0;
+    if (more) blk = Block(w, p, b, kDeepApply, V);
+#pragma unroll
+    for (int u = 0; u < kDeepApply; ++u, out += out_step) {
+      float v[V];
+      widen<T>(raw[u], v);
+      if (more) load(u);
+      one(v, V, o + (int64_t)u * step, out);
+    }
+    if (!more) break;
+  }
+}
+
+// ------------------------------------------------------------------ small maps
+// A workgroup takes cw channels (whole groups) of a sample and holds all their pixels in registers: one
+// launch, every value read once.  Bound by latency.
+constexpr int kSmall = 512;       // threads
+constexpr int kSmallHold = 16;    // vectors of x that a thread holds, in the backward kSmallHold / 2 of x and of dy
+struct Slice {
+  int64_t P;         // pixels
+  int32_t C, D, G;   // channels, a group's, groups
+  int32_t cw, S, RS; // channels, 16-byte slots and rows side by side of a workgroup
+  int32_t nv;        // vectors that a thread holds
+};
+struct SliceSpot {
+  int n, c0, rr, slot, c;  // sample, first channel, row, slot, the thread's first channel
+  bool active;
+  __device__ __forceinline__ SliceSpot(const Slice& w, int V) {
+    const int per = w.C / w.cw, b = blockIdx.x, t = threadIdx.x;
+    n = b / per;
+    c0 = (b - n * per) * w.cw;
+    rr = t / w.S;
+    slot = t - rr * w.S;
+    active = rr < w.RS;
+    c = c0 + slot * V;
+  }
+};
+// f(group of the workgroup, sums of v over its threads), v per thread (D % V == 0: one group's).
+template <typename F>
+__device__ __forceinline__ void slice_sums(const Slice& w, int V, float2 v, float2* s, F&& f) {
+  const int gw = w.cw / w.D, DE = w.D / V, Q = sharers(gw, kSmall), lane = threadIdx.x & (Q - 1);
+  s[threadIdx.x] = v;
+  __syncthreads();
+#pragma unroll 1
+  for (int g = threadIdx.x / Q; g < gw; g += kSmall / Q) {
+    float2 a = make_float2(0.0f, 0.0f);
+    auto add = [&](float2 t) {
+      a.x += t.x;
+      a.y += t.y;
+    };
+    if (w.RS >= DE) {
+      for (int e = g * DE; e < (g + 1) * DE; ++e)
+        for (int r = lane; r < w.RS; r += Q) add(s[r * w.S + e]);
+    } else {
+      for (int r = 0; r < w.RS; ++r)
+        for (int e = g * DE + lane; e < (g + 1) * DE; e += Q) add(s[r * w.S + e]);
+    }
+    a.x = lanes_sum(a.x, Q);
+    a.y = lanes_sum(a.y, Q);
+    if (lane == 0) f(g, a);
+  }
+  __syncthreads();
+}
+
+template <typename T, int ACT, int MODE>
+__global__ __launch_bounds__(kSmall) void gn_small_kernel(const T* __restrict__ x, Slice w, Affine f, float eps,
+                                                          float* mean_out, float* rstd_out, T* __restrict__ y,
+                                                          int8_t* __restrict__ q, uint8_t* __restrict__ scale) {
+  constexpr int V = Vec<T>::V;
+  __shared__ float2 s[kSmall];
+  __shared__ float s_mu[kSmall], s_rs[kSmall];
+  const SliceSpot p(w, V);
+  const int64_t base = (int64_t)p.n * w.P * w.C + p.c;
+  u32x4 raw[kSmallHold];
+#pragma unroll
+  for (int i = 0; i < kSmallHold; ++i)
+    if (i < w.nv) {
+      const int64_t r = p.rr + (int64_t)i * w.RS;
+      raw[i] = u32x4{};
+      if (p.active && r < w.P) raw[i] = load_raw(x + base + r * w.C);
+    }
+  float a[V], b[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    a[j] = load_param(f.weight, f.type, p.c + j, 1.0f);
+    b[j] = load_param(f.bias, f.type, p.c + j, 0.0f);
+  }
+  // a mean of plain sums, and from the distances to it its error and the spread: exact to fp32 wherever
+  // the mean lies
+  float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+  for (int i = 0; i < kSmallHold; ++i)
+    if (i < w.nv) {
+      float v[V];
+      widen<T>(raw[i], v);
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum.x += v[j];
+    }
+  const float cnt = (float)(w.P * w.D);
+  slice_sums(w, V, sum, s, [&](int g, float2 t) { s_mu[g] = t.x / cnt; });
+  const int gl = (p.c - p.c0) / w.D;
+  const float mu0 = s_mu[gl];
+  sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+  for (int i = 0; i < kSmallHold; ++i)
+    if (i < w.nv) {
+      float v[V];
+      widen<T>(raw[i], v);
+      const bool in = p.active && p.rr + (int64_t)i * w.RS < w.P;
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float d = in ? v[j] - mu0 : 0.0f;
+        sum.x += d;
+        sum.y = fmaf(d, d, sum.y);
       }
     }
-  }
+  slice_sums(w, V, sum, s, [&](int g, float2 t) {
+    const double e = (double)t.x / cnt, var = (double)t.y / cnt - e * e;
+    const float r = (float)(1.0 / sqrt((var < 0.0 ? 0.0 : var) + (double)eps));  // keeps a NaN
+    s_mu[g] = (float)(s_mu[g] + e);
+    s_rs[g] = r;
+    if (mean_out) {
+      const int i = p.n * w.G + p.c0 / w.D + g;
+      mean_out[i] = s_mu[g];
+      rstd_out[i] = r;
+    }
+  });
+  const float mu = s_mu[gl];
+  const float rs = s_rs[gl];
+#pragma unroll
+  for (int j = 0; j < V; ++j) a[j] *= rs;
+#pragma unroll
+  for (int i = 0; i < kSmallHold; ++i)
+    if (i < w.nv) {
+      const int64_t r = p.rr + (int64_t)i * w.RS;
+      const bool in = p.active && r < w.P;
+      float v[V];
+      widen<T>(raw[i], v);
+      const int64_t o = base + r * w.C;
+      if constexpr (MODE == kCheckpoint) {  // cw % 32 == 0: a block is 32 channels of a pixel
+        int sc;
+        const auto bytes = quantise_vec<V>(v, sc);
+        if (in) {
+          *reinterpret_cast<typename Bytes<V>::type*>(q + o) = bytes;
+          if (p.slot % (kBlock8 / V) == 0) scale[o / kBlock8] = (uint8_t)sc;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = act_fwd<ACT, T>(fmaf(v[j] - mu, a[j], b[j]));
+      if (!in) continue;
+      if constexpr (MODE == kPacked) store_vec(y + (int64_t)p.n * w.P * w.C + ((p.c / V) * w.P + r) * V, v);
+      else store_vec(y + o, v);
+    }
 }
 
 // ------------------------------------------------------------------ backward
@@ -621,30 +771,61 @@ struct Source {
   int in_block;
 };
 template <typename T, bool Q8>
-struct Held {  // V of them
-  u32x4 v;
-  __device__ __forceinline__ void load(const Source<T, Q8>& x, int64_t o, uint32_t off) { v = load_raw(at(x.x + o, off)); }
-  __device__ __forceinline__ void get(float (&out)[Vec<T>::V]) const { widen<T>(v, out); }
+struct Pair {  // V values of x and of dy in flight
+  u32x4 xs, d;
+  __device__ __forceinline__ void load(const Source<T, Q8>& x, const T* dy, int64_t o, uint32_t off) {
+    xs = load_raw(at(x.x + o, off));
+    d = load_raw(at(dy + o, off));
+  }
+  __device__ __forceinline__ void get(const Source<T, Q8>&, float (&v)[Vec<T>::V], float (&dv)[Vec<T>::V]) const {
+    widen<T>(xs, v);
+    widen<T>(d, dv);
+  }
 };
 template <typename T>
-struct Held<T, true> {  // whole ones need Source::in_block
-  typename Bytes<Vec<T>::V>::type q;
-  int scale;
-  __device__ __forceinline__ void load(const Source<T, true>& x, int64_t o, uint32_t off) {
-    q = *reinterpret_cast<const typename Bytes<Vec<T>::V>::type*>(at(x.q + o, off));
-    scale = x.scale[(o + off) / kBlock8];
+struct Pair<T, true> {
+  static constexpr int V = Vec<T>::V;
+  typename Bytes<V>::type q;
+  int s0, s1;  // the scales of the values before and from `cut` on
+  int cut;
+  u32x4 d;
+  __device__ __forceinline__ void load(const Source<T, true>& x, const T* dy, int64_t o, uint32_t off) {
+    const int64_t i = o + off;
+    if (x.in_block) {
+      q = *reinterpret_cast<const typename Bytes<V>::type*>(at(x.q + o, off));
+      s0 = x.scale[i / kBlock8];
+    } else {  // at any byte, over two blocks
+      typedef typename Bytes<V>::type Any __attribute__((aligned(1)));
+      q = *reinterpret_cast<const Any*>(at(x.q + o, off));
+      s0 = x.scale[i / kBlock8];
+      s1 = x.scale[(i + V - 1) / kBlock8];
+      cut = kBlock8 - (int)(i % kBlock8);
+    }
+    d = load_raw(at(dy + o, off));
   }
-  __device__ __forceinline__ void get(float (&out)[Vec<T>::V]) const { restore_vec<Vec<T>::V>(q, step_of(scale), out); }
+  __device__ __forceinline__ void get(const Source<T, true>& x, float (&v)[V], float (&dv)[V]) const {
+    if (x.in_block) {
+      restore_vec<V>(q, step_of(s0), v);
+    } else {
+      restore_vec<V>(q, 1.0f, v);
+      const float a = step_of(s0), b = step_of(s1);
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] *= j < cut ? a : b;
+    }
+    widen<T>(d, dv);
+  }
 };
 // The first m values one by one, zeros behind them.
 template <typename T, bool Q8>
-__device__ __forceinline__ void values(const Source<T, Q8>& x, int64_t i, int m, float (&v)[Vec<T>::V]) {
+__device__ __forceinline__ void first_values(const Source<T, Q8>& x, const T* dy, int64_t i, int m, float (&v)[Vec<T>::V],
+                                             float (&d)[Vec<T>::V]) {
 #pragma unroll
   for (int j = 0; j < Vec<T>::V; ++j) {
-    v[j] = 0.0f;
+    v[j] = d[j] = 0.0f;
     if (j < m) {
       if constexpr (Q8) v[j] = (float)x.q[i + j] * step_of(x.scale[(i + j) / kBlock8]);
       else v[j] = (float)x.x[i + j];
+      d[j] = (float)dy[i + j];
     }
   }
 }
@@ -686,31 +867,28 @@ __global__ __launch_bounds__(kThreads) void gn_grad_sums_kernel(const T* __restr
 #pragma unroll 1
   for (int b = p.part; b < w.blocks; b += w.parts) {
     const Block blk(w, p, b, kDeepSums, V);
-    if (blk.whole == kDeepSums && (!Q8 || x.in_block)) {
-      u32x4 hd[kDeepSums];
-      Held<T, Q8> hx[kDeepSums];
+    Pair<T, Q8> h[kDeepSums];
+    float v[V], d[V];
+    if (blk.whole == kDeepSums) {
+#pragma unroll
+      for (int u = 0; u < kDeepSums; ++u) h[u].load(x, dy, blk.at + (int64_t)u * step, p.off);
 #pragma unroll
       for (int u = 0; u < kDeepSums; ++u) {
-        hx[u].load(x, blk.at + (int64_t)u * step, p.off);
-        hd[u] = load_raw(at(dy + blk.at + (int64_t)u * step, p.off));
-      }
-#pragma unroll
-      for (int u = 0; u < kDeepSums; ++u) {
-        float v[V], d[V];
-        hx[u].get(v);
-        widen<T>(hd[u], d);
+        h[u].get(x, v, d);
         add(v, d, V);
       }
-    } else {
-#pragma unroll 1
-      for (int u = 0; u < kDeepSums && u <= blk.whole; ++u) {
-        const int m = u < blk.whole ? V : blk.tail;
-        const int64_t o = blk.at + (int64_t)u * step + p.off;
-        float v[V], d[V];
-        values(x, o, m, v);
-        widen<T>(load_first(dy + o, m), d);
-        add(v, d, m);
-      }
+    } else {  // the sample's last block
+#pragma unroll
+      for (int u = 0; u < kDeepSums - 1; ++u)
+        if (u < blk.whole) h[u].load(x, dy, blk.at + (int64_t)u * step, p.off);
+      first_values(x, dy, blk.at + (int64_t)blk.whole * step + p.off, blk.tail, v, d);
+      add(v, d, blk.tail);
+#pragma unroll
+      for (int u = 0; u < kDeepSums - 1; ++u)
+        if (u < blk.whole) {
+          h[u].get(x, v, d);
+          add(v, d, V);
+        }
     }
   }
 #pragma unroll
@@ -823,6 +1001,10 @@ struct Params {  // of the parameters' gradients: the first `blocks` workgroups 
   int32_t blocks;
 };
 
+__global__ __launch_bounds__(kThreads) void gn_param_grads_kernel(Params pg, int C, int type) {
+  param_grads(pg.pos, pg.rows, C, type, pg.dweight, pg.dbias, blockIdx.x);
+}
+
 // dx = a g - rstd E[weight g] - (x - mean) rstd^2 E[weight g xhat], a = rstd * weight.
 template <typename T, int ACT, bool Q8>
 __global__ __launch_bounds__(kThreads) void gn_grad_input_kernel(const T* __restrict__ dy, Source<T, Q8> x, Walk w,
@@ -837,19 +1019,13 @@ __global__ __launch_bounds__(kThreads) void gn_grad_input_kernel(const T* __rest
   }
   const Place p(w, V, blockIdx.x - pg.blocks);
   const int step = w.RS * w.Cv;
-  const bool vectors = !Q8 || x.in_block;
   int b = w.blocks - 1 - p.part;  // backwards and ahead, as gn_apply_kernel
-  u32x4 hd[kDeepGrad];
-  Held<T, Q8> hx[kDeepGrad];
+  Pair<T, Q8> h[kDeepGrad];
   Block blk(w, p, b, kDeepGrad, V);
-  auto load = [&](int u) {
-    hx[u].load(x, blk.at + (int64_t)u * step, p.off);
-    hd[u] = load_raw(at(dy + blk.at + (int64_t)u * step, p.off));
-  };
-  if (vectors && blk.whole == kDeepGrad) {
+  auto load = [&](int u) { h[u].load(x, dy, blk.at + (int64_t)u * step, p.off); };
 #pragma unroll
-    for (int u = 0; u < kDeepGrad; ++u) load(u);
-  }
+  for (int u = 0; u < kDeepGrad; ++u)
+    if (u < blk.whole) load(u);
   if (rec) {
     const int Q = sharers(w.G), lane = threadIdx.x & (Q - 1);
 #pragma unroll 1
@@ -877,40 +1053,148 @@ __global__ __launch_bounds__(kThreads) void gn_grad_input_kernel(const T* __rest
       v[j] = fmaf(-xc, m2[j], fmaf(k.a[j], g, -m1[j]));
     }
   };
-#pragma unroll 1
-  while (b >= 0) {
-    const int64_t o = blk.at;
-    const int whole = blk.whole, tail = blk.tail;
+  if (blk.whole < kDeepGrad) {  // the sample's last block
+    float v[V], d[V];
+#pragma unroll
+    for (int u = 0; u < kDeepGrad - 1; ++u)
+      if (u < blk.whole) {
+        h[u].get(x, v, d);
+        grad(v, d);
+        if (p.active) store_vec(at(dx + blk.at + (int64_t)u * step, p.off), v);
+      }
+    const int64_t i = blk.at + (int64_t)blk.whole * step + p.off;
+    first_values(x, dy, i, blk.tail, v, d);
+    grad(v, d);
+    if (p.active) store_first(dx + i, v, blk.tail);
     b -= w.parts;
-    if (b >= 0) blk = Block(w, p, b, kDeepGrad, V);  // a block before another: whole
-    if (vectors && whole == kDeepGrad) {
-      T* out = dx + o;
+    if (b < 0) return;
+    blk = Block(w, p, b, kDeepGrad, V);
 #pragma unroll
-      for (int u = 0; u < kDeepGrad; ++u, out += step) {
-        float v[V], d[V];
-        hx[u].get(v);
-        widen<T>(hd[u], d);
-        if (b >= 0) load(u);
-        grad(v, d);
-        if (p.active) store_vec(at(out, p.off), v);
-      }
-    } else {
+    for (int u = 0; u < kDeepGrad; ++u) load(u);
+  }
 #pragma unroll 1
-      for (int u = 0; u < kDeepGrad && u <= whole; ++u) {
-        const int m = u < whole ? V : tail;
-        const int64_t i = o + (int64_t)u * step + p.off;
-        float v[V], d[V];
-        values(x, i, m, v);
-        widen<T>(load_first(dy + i, m), d);
-        grad(v, d);
-        if (p.active) store_first(dx + i, v, m);
-      }
-      if (vectors && b >= 0) {
+  for (;;) {
+    T* out = dx + blk.at;
+    b -= w.parts;
+    const bool more = b >= 0;
+    if (more) blk = Block(w, p, b, kDeepGrad, V);
 #pragma unroll
-        for (int u = 0; u < kDeepGrad; ++u) load(u);
+    for (int u = 0; u < kDeepGrad; ++u, out += step) {
+      float v[V], d[V];
+      h[u].get(x, v, d);
+      if (more) load(u);
+      grad(v, d);
+      if (p.active) store_vec(at(out, p.off), v);
+    }
+    if (!more) break;
+  }
+}
+
+// The backward of gn_small_kernel.  pos [N][C]: (sum g, sum g xhat); with one sample, dweight and dbias.
+template <typename T, int ACT, bool Q8>
+__global__ __launch_bounds__(kSmall) void gn_small_grad_kernel(const T* __restrict__ dy, Source<T, Q8> x, Slice w, Affine f,
+                                                               float2* __restrict__ pos, void* dweight, void* dbias,
+                                                               T* __restrict__ dx) {
+  constexpr int V = Vec<T>::V;
+  __shared__ float s_1[kSmall * V], s_2[kSmall * V], s_m1[kSmall], s_m2[kSmall];
+  const SliceSpot p(w, V);
+  const int64_t base = (int64_t)p.n * w.P * w.C + p.c0;
+  const uint32_t off = (p.active ? p.rr * w.C : 0) + (p.active ? p.slot * V : 0);
+  const int64_t step = (int64_t)w.RS * w.C;
+  Pair<T, Q8> h[kSmallHold / 2];
+#pragma unroll
+  for (int i = 0; i < kSmallHold / 2; ++i)
+    if (i < w.nv && p.active && p.rr + (int64_t)i * w.RS < w.P) h[i].load(x, dy, base + i * step, off);
+  const int g0 = p.n * w.G + (p.active ? p.c : p.c0) / w.D;
+  const float mu = f.mean[g0], rs = f.rstd[g0];
+  float a[V], b[V], s1[V] = {}, s2[V] = {};
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int c = p.active ? p.c + j : p.c0;
+    a[j] = rs * load_param(f.weight, f.type, c, 1.0f);
+    b[j] = load_param(f.bias, f.type, c, 0.0f);
+  }
+#pragma unroll
+  for (int i = 0; i < kSmallHold / 2; ++i)
+    if (i < w.nv && p.active && p.rr + (int64_t)i * w.RS < w.P) {
+      float v[V], d[V];
+      h[i].get(x, v, d);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float xc = v[j] - mu, g = d[j] * act_slope<ACT>(fmaf(xc, a[j], b[j]));
+        s1[j] += g;
+        s2[j] = fmaf(g, xc, s2[j]);
+      }
+    }
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    s_1[threadIdx.x * V + j] = s1[j];
+    s_2[threadIdx.x * V + j] = s2[j];
+  }
+  __syncthreads();
+  {
+    const int L = sharers(w.cw, kSmall), lane = threadIdx.x & (L - 1);
+#pragma unroll 1
+    for (int i = threadIdx.x / L; i < w.cw; i += kSmall / L) {
+      float t1 = 0.0f, t2 = 0.0f;
+#pragma unroll 1
+      for (int r = lane; r < w.RS; r += L) {
+        t1 += s_1[r * w.cw + i];
+        t2 += s_2[r * w.cw + i];
+      }
+      t1 = lanes_sum(t1, L);
+      t2 = lanes_sum(t2, L);
+      if (lane == 0) {
+        const int c = p.c0 + i;
+        t2 *= f.rstd[p.n * w.G + c / w.D];
+        if (pos) {
+          pos[(int64_t)p.n * w.C + c] = make_float2(t1, t2);
+        } else {
+          if (dbias) store_param(dbias, f.type, c, t1);
+          if (dweight) store_param(dweight, f.type, c, t2);
+        }
+        const float wt = load_param(f.weight, f.type, c, 1.0f);
+        s_1[i] = wt * t1;  // row 0's place, which only these lanes have read
+        s_2[i] = wt * t2;
       }
     }
   }
+  if (!dx) return;
+  __syncthreads();
+  {
+    const int gw = w.cw / w.D, Q = sharers(gw, kSmall), lane = threadIdx.x & (Q - 1);
+#pragma unroll 1
+    for (int g = threadIdx.x / Q; g < gw; g += kSmall / Q) {
+      float m1 = 0.0f, m2 = 0.0f;
+#pragma unroll 1
+      for (int i = g * w.D + lane; i < (g + 1) * w.D; i += Q) {
+        m1 += s_1[i];
+        m2 += s_2[i];
+      }
+      m1 = lanes_sum(m1, Q);
+      m2 = lanes_sum(m2, Q);
+      if (lane == 0) {
+        const float r = f.rstd[p.n * w.G + p.c0 / w.D + g], each = r / (float)(w.P * w.D);
+        s_m1[g] = each * m1;
+        s_m2[g] = each * r * m2;
+      }
+    }
+  }
+  __syncthreads();
+  const int gl = p.active ? (p.c - p.c0) / w.D : 0;
+  const float m1 = s_m1[gl], m2 = s_m2[gl];
+#pragma unroll
+  for (int i = 0; i < kSmallHold / 2; ++i)
+    if (i < w.nv && p.active && p.rr + (int64_t)i * w.RS < w.P) {
+      float v[V], d[V];
+      h[i].get(x, v, d);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float xc = v[j] - mu, g = d[j] * act_slope<ACT>(fmaf(xc, a[j], b[j]));
+        v[j] = fmaf(-xc, m2, fmaf(a[j], g, -m1));
+      }
+      store_vec(at(dx + base + i * step, off), v);
+    }
 }
 
 // ------------------------------------------------------------------ host side
@@ -970,6 +1254,29 @@ unsigned grid_for(int type, int64_t n) {
   return (unsigned)std::min<int64_t>((n + per - 1) / per, int64_t(1) << 20);
 }
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+// The small maps' cut, or cw = 0: whole groups of whole vectors, as few as hold 32 channels, whose pixels
+// a workgroup can hold.
+Slice make_slice(const DpftGroupNorm& d, int hold) {
+  Slice w{};
+  const int V = d.x_type == DPFT_TYPE_F32 ? 4 : 8, D = d.C / d.groups;
+  if (D % V || d.C > (1 << 16)) return w;
+  int gw = 1;
+  while (gw < d.groups && (gw * D < 32 || d.groups % gw)) ++gw;
+  const int cw = gw * D, S = cw / V;
+  if (S > kSmall) return w;
+  const int RS = kSmall / S;
+  if (d.pixels > (int64_t)RS * hold) return w;
+  w.P = d.pixels;
+  w.C = d.C;
+  w.D = D;
+  w.G = d.groups;
+  w.cw = cw;
+  w.S = S;
+  w.RS = RS;
+  w.nv = (int)((d.pixels + RS - 1) / RS);
+  return w;
+}
+
 // The workspace: the forward's records, then statistics that nobody asked for; the backward's records,
 // positions and, for many groups, means.
 size_t record_bytes(const Walk& w, size_t one) { return round256((size_t)w.N * w.parts * w.tiles * w.G * one); }
@@ -977,6 +1284,7 @@ size_t position_bytes(const Walk& w) { return round256((size_t)w.N * w.parts * w
 size_t group_bytes(const Walk& w) { return round256((size_t)w.N * w.G * sizeof(float2)); }
 size_t need(const DpftGroupNorm& d) {
   const Walk f = make_walk(d, kDeep, kStatsWorkgroups), b = make_walk(d, kDeepSums, kSumsWorkgroups);
+  // (positions: at least a row of C a sample, which is what the small maps' backward needs)
   return std::max(record_bytes(f, sizeof(float4)) + group_bytes(f),
                   record_bytes(b, sizeof(float2)) + position_bytes(b) + group_bytes(b));
 }
@@ -989,6 +1297,12 @@ bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
 template <typename T, int ACT, int MODE>
 void launch_forward(const DpftGroupNorm& d, const T* x, Affine f, float* mean_out, float* rstd_out, T* y, int8_t* q,
                     uint8_t* scale, void* ws, hipStream_t st) {
+  const Slice sl = make_slice(d, kSmallHold);
+  if (sl.cw) {
+    hipLaunchKernelGGL((gn_small_kernel<T, ACT, MODE>), dim3((unsigned)(d.N * (d.C / sl.cw))), dim3(kSmall), 0, st, x, sl, f,
+                       d.eps, mean_out, rstd_out, y, q, scale);
+    return;
+  }
   const Walk ws1 = make_walk(d, kDeep, kStatsWorkgroups), w = make_walk(d, kDeepApply, kApplyWorkgroups);
   const int R = ws1.parts * ws1.tiles;
   const dim3 block(kThreads);
@@ -1012,15 +1326,24 @@ template <typename T, int ACT, bool Q8>
 void launch_backward(const DpftGroupNorm& d, const T* dy, Source<T, Q8> x, const Affine& f, T* dx, void* dweight,
                      void* dbias, void* ws, hipStream_t st) {
   const Walk ws1 = make_walk(d, kDeepSums, kSumsWorkgroups), w = make_walk(d, kDeepGrad, kGradWorkgroups);
-  const int R = ws1.parts * ws1.tiles;
+  const int R = ws1.parts * ws1.tiles, param_blocks = dweight || dbias ? (d.C + kGradCh - 1) / kGradCh : 0;
   const dim3 block(kThreads);
   x.in_block = w.in_block;
   float2* rec = static_cast<float2*>(ws);
+  const Slice sl = make_slice(d, kSmallHold / 2);
+  if (sl.cw) {
+    float2* rows = d.N > 1 && param_blocks ? rec : nullptr;
+    hipLaunchKernelGGL((gn_small_grad_kernel<T, ACT, Q8>), dim3((unsigned)(d.N * (d.C / sl.cw))), dim3(kSmall), 0, st, dy, x,
+                       sl, f, rows, d.N > 1 ? nullptr : dweight, d.N > 1 ? nullptr : dbias, dx);
+    if (rows)
+      hipLaunchKernelGGL(gn_param_grads_kernel, dim3((unsigned)param_blocks), block, 0, st,
+                         Params{rows, d.N, dweight, dbias, param_blocks}, d.C, d.param_type);
+    return;
+  }
   float2* pos = reinterpret_cast<float2*>(static_cast<char*>(ws) + record_bytes(ws1, sizeof(float2)));
   float2* means = reinterpret_cast<float2*>(reinterpret_cast<char*>(pos) + position_bytes(ws1));
   hipLaunchKernelGGL((gn_grad_sums_kernel<T, ACT, Q8>), dim3(walk_grid(ws1)), block, 0, st, dy, x, ws1, f, pos, rec);
-  const Params pg{pos, (int64_t)d.N * ws1.parts * (w.Cv / w.C), dweight, dbias,
-                  dweight || dbias ? (w.C + kGradCh - 1) / kGradCh : 0};
+  const Params pg{pos, (int64_t)d.N * ws1.parts * (w.Cv / w.C), dweight, dbias, param_blocks};
   if (dx && !fold(ws1)) {
     hipLaunchKernelGGL(gn_finish_grads_kernel, dim3(waves_grid((int64_t)d.N * d.groups)), block, 0, st, rec, R, w, f, means);
     rec = nullptr;
@@ -1066,6 +1389,10 @@ int dpft_group_norm_act(const DpftGroupNorm* desc, const void* x, const void* we
   if (misaligned(x) || misaligned(y) || misaligned(ws) || misaligned(q_out) || misaligned(scale_out))
     return dpft_fail(DPFT_E_INVALID, "x, y, the checkpoint and the workspace must be 16-byte aligned");
   const Walk w = make_walk(d, kDeepApply, kApplyWorkgroups);
+  const Slice sl = make_slice(d, kSmallHold);
+  // written with y where a checkpoint's blocks are whole lanes of a workgroup; else by a pass of its own:
+  // y is the same either way
+  const bool with_y = q_out && (sl.cw ? sl.cw % kBlock8 == 0 : w.lanes_block != 0);
   if (ws_bytes < need(d)) return dpft_fail(DPFT_E_WORKSPACE, "workspace %zu < %zu", ws_bytes, need(d));
   hipStream_t st = static_cast<hipStream_t>(hip_stream);
   const Affine f{weight, bias, nullptr, nullptr, d.param_type};
@@ -1078,14 +1405,13 @@ int dpft_group_norm_act(const DpftGroupNorm* desc, const void* x, const void* we
       if (d.flags & DPFT_GN_PACKED)
         return launch_forward<T, A, kPacked>(d, xs, f, mean_out, rstd_out, ys, nullptr, nullptr, ws, st);
     }
-    if (q_out && w.lanes_block)
+    if (with_y)
       launch_forward<T, A, kCheckpoint>(d, xs, f, mean_out, rstd_out, ys, q_out, scale_out, ws, st);
     else
       launch_forward<T, A, kPlain>(d, xs, f, mean_out, rstd_out, ys, nullptr, nullptr, ws, st);
   });
   if (const int rc = dpft_hip_check("gn_apply_kernel")) return rc;
-  // blocks that cross a thread's values or a workgroup's rows: a pass of their own
-  return q_out && !w.lanes_block ? dpft_act_checkpoint(x, d.x_type, d.N * w.L, q_out, scale_out, hip_stream) : DPFT_OK;
+  return q_out && !with_y ? dpft_act_checkpoint(x, d.x_type, d.N * w.L, q_out, scale_out, hip_stream) : DPFT_OK;
 }
 
 int dpft_group_norm_act_backward(const DpftGroupNorm* desc, const void* dy, const void* x, const int8_t* q,
