@@ -280,7 +280,7 @@ struct Walk {
 };
 
 // Vectors of a block, which a thread has in flight: of the statistics, of the apply pass, of the backward's two.
-constexpr int kDeep = 8, kDeepApply = 4, kDeepSums = 2, kDeepGrad = 2;
+constexpr int kDeep = 8, kDeepApply = 4, kDeepSums = 4, kDeepGrad = 2;
 
 struct Place {
   int n, part, tile, slot, rr;
@@ -334,25 +334,25 @@ __device__ __forceinline__ F lanes_sum(F v, int q) {
   for (int o = q >> 1; o > 0; o >>= 1) v += __shfl_xor(v, o);
   return v;
 }
+// f(i) by Q lanes over `rows` x `n` entries r * row + i, i < n, in a fixed order.
+template <typename F>
+__device__ __forceinline__ void over_box(int rows, int row, int n, int lane, int Q, F&& f) {
+  const uint32_t by_n = n > 1 ? 0xffffffffu / (uint32_t)n + 1 : 0;  // r = e / n, exact for e n < 2^32
+#pragma unroll 4
+  for (int e = lane; e < rows * n; e += Q) {
+    const int r = n > 1 ? (int)__umulhi((uint32_t)e, by_n) : e;
+    f(r * row + (e - r * n));
+  }
+}
 // f(i) by Q lanes over the entries i of group g in shared memory that lie in a tile: an entry for each
-// `per` values of a tile's row, RS rows.  The lanes share the longer of rows and entries of a row.
+// `per` values of a tile's row, RS rows.
 template <typename F>
 __device__ __forceinline__ void over_entries(const Walk& w, int tile, int V, int per, int g, int lane, int Q, F&& f) {
   const int lo = tile * w.W * V, hi = min(lo + w.W * V, w.Cv), RE = w.W * V / per;
 #pragma unroll 1
   for (int k = g * w.D; k < hi; k += w.C) {  // the row's copies of the group's channels
     const int e0 = (max(k, lo) - lo) / per, e1 = (min(k + w.D, hi) - lo) / per;
-    if (w.RS >= e1 - e0) {
-#pragma unroll 1
-      for (int e = e0; e < e1; ++e)
-#pragma unroll 1
-        for (int r = lane; r < w.RS; r += Q) f(r * RE + e);
-    } else {
-#pragma unroll 1
-      for (int r = 0; r < w.RS; ++r)
-#pragma unroll 1
-        for (int e = e0 + lane; e < e1; e += Q) f(r * RE + e);
-    }
+    if (e1 > e0) over_box(w.RS, RE, e1 - e0, lane, Q, [&](int i) { f(e0 + i); });
   }
 }
 
@@ -536,6 +536,13 @@ __global__ __launch_bounds__(kThreads) void gn_apply_kernel(const T* __restrict_
   for (int u = 0; u < kDeepApply; ++u)
     if (u < blk.whole) load(u);
   if (blk.whole < kDeepApply) end = load_first(at(x + blk.at + (int64_t)blk.whole * step, p.off), blk.tail);
+  float mu[V], a[V], bias[V];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int c0 = p.channel + j, c = c0 < w.C ? c0 : c0 % w.C;
+    a[j] = load_param(f.weight, f.type, c, 1.0f);
+    bias[j] = load_param(f.bias, f.type, c, 0.0f);
+  }
   if (rec) {
     const int Q = sharers(w.G), lane = threadIdx.x & (Q - 1);
 #pragma unroll 1
@@ -552,13 +559,11 @@ __global__ __launch_bounds__(kThreads) void gn_apply_kernel(const T* __restrict_
     }
     __syncthreads();
   }
-  float mu[V], a[V], bias[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
-    const int c0 = p.channel + j, c = c0 < w.C ? c0 : c0 % w.C, g = c / w.D;
+    const int c0 = p.channel + j, g = (c0 < w.C ? c0 : c0 % w.C) / w.D;
     mu[j] = rec ? s_mu[g] : f.mean[p.n * w.G + g];
-    a[j] = (rec ? s_rs[g] : f.rstd[p.n * w.G + g]) * load_param(f.weight, f.type, c, 1.0f);
-    bias[j] = load_param(f.bias, f.type, c, 0.0f);
+    a[j] *= rec ? s_rs[g] : f.rstd[p.n * w.G + g];
   }
   // in the channel-quad layout a slot's rows follow one another
   const int out_step = MODE == kPacked ? w.RS * V : step;
@@ -656,13 +661,7 @@ __device__ __forceinline__ void slice_sums(const Slice& w, int V, float2 v, floa
       a.x += t.x;
       a.y += t.y;
     };
-    if (w.RS >= DE) {
-      for (int e = g * DE; e < (g + 1) * DE; ++e)
-        for (int r = lane; r < w.RS; r += Q) add(s[r * w.S + e]);
-    } else {
-      for (int r = 0; r < w.RS; ++r)
-        for (int e = g * DE + lane; e < (g + 1) * DE; e += Q) add(s[r * w.S + e]);
-    }
+    over_box(w.RS, w.S, DE, lane, Q, [&](int i) { add(s[g * DE + i]); });
     a.x = lanes_sum(a.x, Q);
     a.y = lanes_sum(a.y, Q);
     if (lane == 0) f(g, a);
@@ -853,8 +852,15 @@ __global__ __launch_bounds__(kThreads) void gn_grad_sums_kernel(const T* __restr
   constexpr int V = Vec<T>::V;
   __shared__ float s_1[kThreads * V], s_2[kThreads * V];
   const Place p(w, V, blockIdx.x);
-  const Coefs<V> k(w, p, f);
   const int step = w.RS * w.Cv;
+  int b = p.part;
+  Pair<T, Q8> h[kDeepSums];
+  Block blk(w, p, b, kDeepSums, V);
+  auto load = [&](int u) { h[u].load(x, dy, blk.at + (int64_t)u * step, p.off); };
+#pragma unroll
+  for (int u = 0; u < kDeepSums; ++u)
+    if (u < blk.whole) load(u);
+  const Coefs<V> k(w, p, f);
   float s1[V] = {}, s2[V] = {};
   auto add = [&](const float(&v)[V], const float(&d)[V], int m) {
 #pragma unroll
@@ -864,32 +870,36 @@ __global__ __launch_bounds__(kThreads) void gn_grad_sums_kernel(const T* __restr
       s2[j] = fmaf(g, xc, s2[j]);
     }
   };
+  // whole blocks, the next one's loads issued as the vectors of this one are used
 #pragma unroll 1
-  for (int b = p.part; b < w.blocks; b += w.parts) {
-    const Block blk(w, p, b, kDeepSums, V);
-    Pair<T, Q8> h[kDeepSums];
+  while (b < w.blocks && blk.whole == kDeepSums) {
+    b += w.parts;
+    const bool more = b < w.blocks;
+    if (more) blk = Block(w, p, b, kDeepSums, V);
+    const bool whole = more && blk.whole == kDeepSums;
+#pragma unroll
+    for (int u = 0; u < kDeepSums; ++u) {
+      float v[V], d[V];
+      h[u].get(x, v, d);
+      if (whole) load(u);
+      add(v, d, V);
+    }
+    if (more && !whole) {
+#pragma unroll
+      for (int u = 0; u < kDeepSums - 1; ++u)
+        if (u < blk.whole) load(u);
+    }
+  }
+  if (b < w.blocks) {  // the sample's last block
     float v[V], d[V];
-    if (blk.whole == kDeepSums) {
+    first_values(x, dy, blk.at + (int64_t)blk.whole * step + p.off, blk.tail, v, d);
+    add(v, d, blk.tail);
 #pragma unroll
-      for (int u = 0; u < kDeepSums; ++u) h[u].load(x, dy, blk.at + (int64_t)u * step, p.off);
-#pragma unroll
-      for (int u = 0; u < kDeepSums; ++u) {
+    for (int u = 0; u < kDeepSums - 1; ++u)
+      if (u < blk.whole) {
         h[u].get(x, v, d);
         add(v, d, V);
       }
-    } else {  // the sample's last block
-#pragma unroll
-      for (int u = 0; u < kDeepSums - 1; ++u)
-        if (u < blk.whole) h[u].load(x, dy, blk.at + (int64_t)u * step, p.off);
-      first_values(x, dy, blk.at + (int64_t)blk.whole * step + p.off, blk.tail, v, d);
-      add(v, d, blk.tail);
-#pragma unroll
-      for (int u = 0; u < kDeepSums - 1; ++u)
-        if (u < blk.whole) {
-          h[u].get(x, v, d);
-          add(v, d, V);
-        }
-    }
   }
 #pragma unroll
   for (int j = 0; j < V; ++j) {
@@ -903,7 +913,7 @@ __global__ __launch_bounds__(kThreads) void gn_grad_sums_kernel(const T* __restr
 #pragma unroll 1
     for (int i = threadIdx.x / P; i < PW; i += kThreads / P) {
       float t1 = 0.0f, t2 = 0.0f;
-#pragma unroll 1
+#pragma unroll 4
       for (int r = pl; r < w.RS; r += P) {
         t1 += s_1[r * PW + i];
         t2 += s_2[r * PW + i];
@@ -1026,6 +1036,7 @@ __global__ __launch_bounds__(kThreads) void gn_grad_input_kernel(const T* __rest
 #pragma unroll
   for (int u = 0; u < kDeepGrad; ++u)
     if (u < blk.whole) load(u);
+  const Coefs<V> k(w, p, f);
   if (rec) {
     const int Q = sharers(w.G), lane = threadIdx.x & (Q - 1);
 #pragma unroll 1
@@ -1038,7 +1049,6 @@ __global__ __launch_bounds__(kThreads) void gn_grad_input_kernel(const T* __rest
     }
     __syncthreads();
   }
-  const Coefs<V> k(w, p, f);
   float m1[V], m2[V];
 #pragma unroll
   for (int j = 0; j < V; ++j) {
@@ -1137,7 +1147,7 @@ __global__ __launch_bounds__(kSmall) void gn_small_grad_kernel(const T* __restri
 #pragma unroll 1
     for (int i = threadIdx.x / L; i < w.cw; i += kSmall / L) {
       float t1 = 0.0f, t2 = 0.0f;
-#pragma unroll 1
+#pragma unroll 4
       for (int r = lane; r < w.RS; r += L) {
         t1 += s_1[r * w.cw + i];
         t2 += s_2[r * w.cw + i];
@@ -1200,7 +1210,7 @@ __global__ __launch_bounds__(kSmall) void gn_small_grad_kernel(const T* __restri
 // ------------------------------------------------------------------ host side
 // Workgroups of the statistics and of the gradients' sums, whose records the others join, and of those
 // that write.  (Statistics, 8 x 32 x 480 x 640 fp32 in all: 512 168 us, 1024 175, 2048 186.)
-constexpr int kStatsWorkgroups = 512, kSumsWorkgroups = 768, kApplyWorkgroups = 1024, kGradWorkgroups = 1024;
+constexpr int kStatsWorkgroups = 512, kSumsWorkgroups = 512, kApplyWorkgroups = 1024, kGradWorkgroups = 1024;
 
 int check(const DpftGroupNorm* d) {
   if (!d) return dpft_fail(DPFT_E_INVALID, "null descriptor");

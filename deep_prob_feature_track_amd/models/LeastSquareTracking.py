@@ -40,11 +40,14 @@ DEFAULT_OPTIONS = dict(vis_feat=False, train_uncer_prop=False, combine_ICP=False
                        feature_channel=1, uncertainty_channel=1, scaler='None', remove_tru_sigma=False,
                        init_pose='identity', train_init_pose=False, scale_init_pose=0.01, multi_hypo='None',
                        res_input=False, checkpoint='')
+# ... and those of this build (the reference's namespaces need not have them): the encoder's
+# normalisation ('batch' or 'group') and, with 'group', 8-bit activation checkpoints in training
+ENCODER_OPTIONS = dict(feature_norm='batch', act_checkpoint=False)
 
 
 def default_options(**overrides):
     """A namespace with every `options` attribute the constructor reads."""
-    d = dict(DEFAULT_OPTIONS)
+    d = dict(DEFAULT_OPTIONS, **ENCODER_OPTIONS)
     d.update(overrides)
     return types.SimpleNamespace(**d)
 
@@ -94,7 +97,10 @@ class LeastSquareTracking(nn.Module):
             self.encoder_type = self.CONV_RGBD if encoder_name == 'ConvRGBD' else self.CONV_RGBD2
             self.encoder = FeaturePyramid(D=4 if encoder_name == 'ConvRGBD' else 8, w_uncertainty=uncertainty_type,
                                           feature_channel=feature_channel, feature_extract=feature_extract,
-                                          uncertainty_channel=uncertainty_channel)
+                                          uncertainty_channel=uncertainty_channel,
+                                          norm=getattr(options, 'feature_norm', ENCODER_OPTIONS['feature_norm']),
+                                          act_checkpoint=getattr(options, 'act_checkpoint',
+                                                                 ENCODER_OPTIONS['act_checkpoint']))
         else:
             raise NotImplementedError()
         self._encoder_nhwc = False  # weights moved to channels_last at the first GPU encode

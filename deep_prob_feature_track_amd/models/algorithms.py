@@ -18,6 +18,8 @@ reference's state_dict keys, so the reference's checkpoints load unchanged:
   algorithms.py:691), PoseNetFeat / PoseNet / SFMPoseNet 1694-1832,
   deep_damping_regressor 1834-1842.
 """
+import functools
+
 import torch
 import torch.nn as nn
 import torch.nn.functional as func
@@ -67,10 +69,14 @@ class FeaturePyramid(nn.Module):
     is repeated to the feature channels as in the reference (1426-1427), as a
     channel-broadcast view (same shape and values, no copy) that the solver wrapper
     recognises and hands to the kernel as one plane (Cs = 1: 2 sigma planes of reads
-    per pixel instead of 2C)."""
+    per pixel instead of 2C).
+    norm='group': group normalisation in every block instead of batch normalisation;
+    act_checkpoint (with it): a training step on the GPU keeps the blocks' activations in 8 bits."""
 
-    def __init__(self, D, w_uncertainty='None', feature_channel=1, feature_extract='conv', uncertainty_channel=1):
+    def __init__(self, D, w_uncertainty='None', feature_channel=1, feature_extract='conv', uncertainty_channel=1,
+                 norm='batch', act_checkpoint=False):
         super().__init__()
+        block = functools.partial(conv, norm=norm, act_checkpoint=act_checkpoint)
         assert uncertainty_channel == feature_channel or uncertainty_channel == 1
         self.w_uncertainty = w_uncertainty != 'None'
         self.uncertainty_type = w_uncertainty
@@ -81,8 +87,8 @@ class FeaturePyramid(nn.Module):
         # backbone: per scale (in, mid, out) with dilations 1, 2, 2
         stages = [(D, 16, 32, 32), (32, 32, 64, 64), (64, 64, 96, 96), (96, 96, 128, 128)]
         for s, (cin, c1, c2, cout) in enumerate(stages):
-            net = nn.Sequential(conv(True, cin, c1, 3), conv(True, c1, c2, 3, dilation=2),
-                                conv(True, c2, cout, 3, dilation=2))
+            net = nn.Sequential(block(True, cin, c1, 3), block(True, c1, c2, 3, dilation=2),
+                                block(True, c2, cout, 3, dilation=2))
             setattr(self, f'net{s}', net)
             initialize_weights(net)
 
@@ -90,7 +96,7 @@ class FeaturePyramid(nn.Module):
             if feature_extract == 'prob_fuse':
                 self.output_C = 16
             if feature_extract in ('conv', 'prob_fuse'):
-                heads = [conv(True, c, self.output_C, kernel_size=1) for c in self.f_channels]
+                heads = [block(True, c, self.output_C, kernel_size=1) for c in self.f_channels]
             elif feature_extract == '1by1':
                 heads = [nn.Conv2d(c, self.output_C, kernel_size=(1, 1)) for c in self.f_channels]
             else:
@@ -101,9 +107,9 @@ class FeaturePyramid(nn.Module):
 
         if self.w_uncertainty and self.uncertainty_type != 'identity':
             if self.uncertainty_type == 'feature':
-                heads = [conv(True, c, self.output_C, 1) for c in self.f_channels]
+                heads = [block(True, c, self.output_C, 1) for c in self.f_channels]
             elif self.uncertainty_type in _UNCERTAINTY_ACTIVATIONS:
-                heads = [nn.Sequential(conv(True, c, 16, kernel_size=1), nn.Conv2d(16, self.uncertainty_C, kernel_size=1))
+                heads = [nn.Sequential(block(True, c, 16, kernel_size=1), nn.Conv2d(16, self.uncertainty_C, kernel_size=1))
                          for c in self.f_channels]
             else:
                 raise NotImplementedError(self.uncertainty_type)

@@ -4,13 +4,17 @@ Restates the reference's code/models/submodules.py (color_normalize 20-23,
 convLayer 25-39, convLayer1d 41-55, fcLayer 57-61, initialize_weights 63-78)
 so that modules built from them carry the reference's state_dict keys:
 a block is nn.Sequential(conv[, batchnorm], ELU) -> keys `<name>.0.weight`,
-`<name>.1.running_mean`, ...
+`<name>.1.running_mean`, ...  A block may have group normalisation instead (norm='group'), whose
+statistics do not depend on the batch: the same in training and in eval mode, at one pair a batch too.
 """
+import math
+
 import torch
 import torch.nn as nn
 from torch.nn import init
 
 from .. import ic
+from .. import norm as gn
 from .. import torch_ops  # noqa: F401  (registers the dpft:: ops torch.compile traces)
 
 _RGB_MEAN = (0.4914, 0.4822, 0.4465)
@@ -42,7 +46,29 @@ class ConvBlock(nn.Sequential):
     In eval mode on the GPU, outside autograd, the batchnorm and the ELU of a 2-D block
     run as one in-place pass over the conv output (`ic.bn_elu_`, dpft_bn_elu) instead of
     two elementwise kernels; otherwise, or for a layout the kernel does not take, the
-    modules run in turn."""
+    modules run in turn.
+    With a GroupNorm, a channels_last map on the GPU goes through `norm.group_norm_act`, in
+    training too; with `act_checkpoint` the backward pass then keeps the conv's input and output
+    in 8 bits (`norm.conv2d`, `group_norm_act(checkpoint=True)`): 2 bytes a value, not 8."""
+
+    act_checkpoint = False
+
+    def _group(self, x):
+        return (len(self) == 3 and isinstance(self[0], nn.Conv2d) and isinstance(self[1], nn.GroupNorm)
+                and isinstance(self[2], nn.ELU) and self[2].alpha == 1.0 and x.is_cuda)
+
+    def _group_conv(self, x):
+        c = self[0]
+        if self.act_checkpoint and torch.is_grad_enabled() and c.padding_mode == 'zeros':
+            return gn.conv2d(x, c.weight, c.bias, c.stride, c.padding, c.dilation, c.groups)
+        return c(x)
+
+    def _group_epilogue(self, y, packed=False):
+        n = self[1]
+        if not y.is_contiguous(memory_format=torch.channels_last):
+            return self[2](n(y))
+        return gn.group_norm_act(y, n.num_groups, n.weight, n.bias, n.eps, "elu", packed=packed,
+                                 checkpoint=self.act_checkpoint)
 
     def _fusable(self, x):
         return (len(self) == 3 and isinstance(self[1], nn.BatchNorm2d) and isinstance(self[2], nn.ELU)
@@ -53,6 +79,10 @@ class ConvBlock(nn.Sequential):
         epilogue can write it (dpft_bn_elu_pack: the batchnorm + ELU of a channels_last
         conv output stored out of place, no separate relayout pass); otherwise forward(x),
         [B,C,H,W].  Same values either way."""
+        if self._group(x) and not torch.is_grad_enabled():
+            y = self[0](x)
+            return self._group_epilogue(y, packed=y.dtype == torch.float32 and y.shape[1] % 4 == 0 and y.is_contiguous(
+                memory_format=torch.channels_last))
         if self._fusable(x):
             y = self[0](x)
             if ic.bn_elu_pack_applies(y, self[1]):
@@ -72,24 +102,41 @@ class ConvBlock(nn.Sequential):
         return self[2](self[1](y))
 
     def forward(self, x):
+        if self._group(x):
+            return self._group_epilogue(self._group_conv(x))
         if self._fusable(x):
             return self._epilogue(self[0](x))
         return super().forward(x)
 
 
-def _block(conv_cls, bn_cls, batch_norm, cin, cout, kernel_size, stride, dilation, bias):
+def _block(conv_cls, norm_fn, batch_norm, cin, cout, kernel_size, stride, dilation, bias):
     layers = [conv_cls(cin, cout, kernel_size=kernel_size, stride=stride,
                        padding=_padding(kernel_size, dilation), dilation=dilation,
                        bias=bias if batch_norm else True)]
     if batch_norm:
-        layers.append(bn_cls(cout))
+        layers.append(norm_fn(cout))
     layers.append(nn.ELU(inplace=True))
     return ConvBlock(*layers)
 
 
-def convLayer(batchNorm, in_planes, out_planes, kernel_size=3, stride=1, dilation=1, bias=False):
-    """Conv2d [+ BatchNorm2d] + ELU."""
-    return _block(nn.Conv2d, nn.BatchNorm2d, batchNorm, in_planes, out_planes, kernel_size, stride, dilation, bias)
+def group_norm(channels):
+    """GroupNorm of 8 groups, or of the most that divide 8 and `channels`."""
+    return nn.GroupNorm(math.gcd(8, channels), channels)
+
+
+_NORMS = {'batch': nn.BatchNorm2d, 'group': group_norm}
+
+
+def convLayer(batchNorm, in_planes, out_planes, kernel_size=3, stride=1, dilation=1, bias=False, norm='batch',
+              act_checkpoint=False):
+    """Conv2d [+ BatchNorm2d, or GroupNorm with norm='group'] + ELU; act_checkpoint (group norm only): ConvBlock."""
+    if norm not in _NORMS:
+        raise ValueError(f"norm must be one of {sorted(_NORMS)} (got {norm!r})")
+    if act_checkpoint and (norm != 'group' or not batchNorm):
+        raise ValueError("act_checkpoint needs norm='group'")
+    block = _block(nn.Conv2d, _NORMS[norm], batchNorm, in_planes, out_planes, kernel_size, stride, dilation, bias)
+    block.act_checkpoint = act_checkpoint
+    return block
 
 
 def convLayer1d(batchNorm, in_planes, out_planes, kernel_size=3, stride=1, dilation=1, bias=False):

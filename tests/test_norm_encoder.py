@@ -1,0 +1,211 @@
+"""Encoder blocks with group normalisation and 8-bit activation checkpoints: the modules on the CPU, and on a
+MI355X (`-m gpu`) the fused blocks against 64 bits and a training step of the whole encoder."""
+import pytest
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+
+import norm_oracle as O
+from deep_prob_feature_track_amd import norm
+from deep_prob_feature_track_amd.models.algorithms import FeaturePyramid
+from deep_prob_feature_track_amd.models.submodules import ConvBlock, convLayer, group_norm
+
+gpu = pytest.mark.gpu
+
+
+def _dev():
+    if not torch.cuda.is_available():
+        pytest.skip("no HIP device")
+    return torch.device("cuda:0")
+
+
+def _jitter(m, seed):
+    g = torch.Generator().manual_seed(seed)
+    with torch.no_grad():
+        for n in m.modules():
+            if isinstance(n, nn.GroupNorm):
+                n.weight.copy_(1 + 0.3 * torch.randn(n.weight.shape, generator=g))
+                n.bias.copy_(0.3 * torch.randn(n.bias.shape, generator=g))
+    return m
+
+
+def _encoder(act_checkpoint=False, seed=0):
+    torch.manual_seed(seed)
+    return _jitter(FeaturePyramid(D=8, w_uncertainty="laplacian", feature_channel=8, feature_extract="conv",
+                                  uncertainty_channel=1, norm="group", act_checkpoint=act_checkpoint), seed)
+
+
+# ------------------------------------------------------------------ without a GPU
+def test_block_options_and_refusals():
+    blk = convLayer(True, 8, 20, 3, norm="group", act_checkpoint=True)
+    assert isinstance(blk, ConvBlock) and isinstance(blk[1], nn.GroupNorm) and blk.act_checkpoint
+    assert blk[1].num_groups == 4 and group_norm(32).num_groups == 8 and group_norm(1).num_groups == 1
+    assert set(blk.state_dict()) == {"0.weight", "1.weight", "1.bias"}
+    assert isinstance(convLayer(True, 8, 16)[1], nn.BatchNorm2d) and not convLayer(True, 8, 16).act_checkpoint
+    with pytest.raises(ValueError):
+        convLayer(True, 8, 16, norm="layer")
+    for kw in (dict(), dict(norm="batch")):
+        with pytest.raises(ValueError):
+            convLayer(True, 8, 16, act_checkpoint=True, **kw)
+    with pytest.raises(ValueError):
+        convLayer(False, 8, 16, norm="group", act_checkpoint=True)
+
+
+def test_cpu_blocks_run_the_modules():
+    """A CPU block is the modules in turn, with gradients and with act_checkpoint (which needs the GPU) too."""
+    blk = _jitter(convLayer(True, 6, 12, 3, norm="group", act_checkpoint=True), 1)
+    seen = []
+    blk[0].register_forward_hook(lambda m, i, o: seen.append(o))  # (two runs of a convolution may differ in a bit)
+    x = torch.randn(2, 6, 9, 11, requires_grad=True)
+    y = blk(x)
+    ref = F.elu(F.group_norm(seen[0], 4, blk[1].weight, blk[1].bias))
+    assert torch.equal(y, ref)
+    assert torch.equal(torch.autograd.grad(y.sum(), seen[0], retain_graph=True)[0],
+                       torch.autograd.grad(ref.sum(), seen[0])[0])
+    z = blk.forward_packed(x)
+    assert torch.equal(z, F.elu(F.group_norm(seen[1], 4, blk[1].weight, blk[1].bias)))
+
+
+def test_encoder_is_the_same_in_training_and_eval_at_any_batch():
+    enc = _encoder()
+    x = torch.randn(3, 8, 16, 24)
+    with torch.no_grad():
+        a = enc.train()(x)
+        b = enc.eval()(x)
+        one = enc(x[1:2])
+    for u, v, w in zip(a[0] + a[1], b[0] + b[1], one[0] + one[1]):
+        assert torch.equal(u, v)
+        # (a convolution of another batch sums in another order: the bound of test_encoder_fused_against_modules)
+        assert (u[1:2] - w).abs().max() <= 20 * 1152 * O.U * w.abs().max()
+    assert not any("running" in k for k in enc.state_dict())
+
+
+def test_tracker_options_reach_the_encoder():
+    from deep_prob_feature_track_amd.models.LeastSquareTracking import LeastSquareTracking, default_options
+    kw = dict(feature_channel=8, uncertainty_channel=1, feature_extract="conv")
+
+    def make(options):
+        return LeastSquareTracking("ConvRGBD2", "laplacian", 3, "None", "Direct-Nodamping", options=options)
+    net = make(default_options(feature_norm="group", act_checkpoint=True, **kw))
+    blocks = [m for m in net.encoder.modules() if isinstance(m, ConvBlock)]
+    assert len(blocks) == 20 and all(isinstance(b[1], nn.GroupNorm) and b.act_checkpoint for b in blocks)
+    plain = default_options(**kw)
+    del plain.feature_norm, plain.act_checkpoint  # the reference's own namespace
+    assert all(isinstance(b[1], nn.BatchNorm2d) for b in make(plain).encoder.modules() if isinstance(b, ConvBlock))
+
+
+# ------------------------------------------------------------------ on the GPU
+@gpu
+@pytest.mark.parametrize("act_checkpoint", [False, True])
+@pytest.mark.parametrize("cin,cout,h,w", [(8, 16, 24, 40), (16, 32, 15, 20), (12, 20, 9, 11)])
+def test_block_in_training_against_64_bits(cin, cout, h, w, act_checkpoint):
+    """conv (1x1) -> group norm -> ELU, forward and backward.  The conv's output is taken as the library's own
+    (its products are not under test); from there the block is the formulas in 64 bits, the checkpoints' rounding
+    among them, with the bounds of norm_oracle; the conv's gradients add their sums' roundings."""
+    dev = _dev()
+    torch.manual_seed(cin + h)
+    blk = _jitter(convLayer(True, cin, cout, 1, norm="group", act_checkpoint=act_checkpoint), 2).to(dev)
+    blk = blk.to(memory_format=torch.channels_last).train()
+    x = torch.randn(2, cin, h, w, device=dev).contiguous(memory_format=torch.channels_last).requires_grad_(True)
+    dy = torch.randn(2, cout, h, w, device=dev).contiguous(memory_format=torch.channels_last)
+    seen = []
+    hook = None if act_checkpoint else blk[0].register_forward_hook(lambda m, i, o: seen.append(o.detach().clone()))
+    y = blk(x)
+    c = norm.conv2d(x, blk[0].weight, None).detach() if act_checkpoint else seen[0]
+    if hook:
+        hook.remove()
+    gx, gw, gn_w, gn_b = torch.autograd.grad(y, (x, blk[0].weight, blk[1].weight, blk[1].bias), dy)
+    r = O.Reference(c, blk[1].num_groups, blk[1].weight, blk[1].bias, blk[1].eps, "elu", dy, checkpoint=act_checkpoint)
+    # c may be a second run of the convolution: cin products, in another order
+    conv_tol = 0.0
+    if act_checkpoint:
+        mag = torch.einsum("oi,nihw->nohw", blk[0].weight.detach().double().abs()[:, :, 0, 0], x.detach().double().abs())
+        conv_tol = float((2 * cin * O.U * mag).max()) * float(r.rstd.max()) * float(blk[1].weight.detach().abs().max())
+    assert O.excess(y, r.y, r.y_tol + 4 * conv_tol) <= 0
+    assert O.excess(gn_b, r.dbias, r.dbias_tol + conv_tol * dy.double().abs().sum((0, 2, 3)) * 4) <= 0
+    xin = x.detach().double()
+    if act_checkpoint:
+        flat = O.through_8_bits(xin.permute(0, 2, 3, 1).reshape(-1))[0]
+        xin = flat.view(2, h, w, cin).permute(0, 3, 1, 2)
+    if not act_checkpoint:  # (a step of an 8-bit value may turn on the last bit of a second convolution)
+        assert O.excess(gn_w, r.dweight, r.dweight_tol * 1.01) <= 0
+        w64 = blk[0].weight.detach().double()[:, :, 0, 0]
+        dw = torch.einsum("nohw,nihw->oi", r.dx, xin)
+        dw_tol = torch.einsum("nohw,nihw->oi", r.dx_tol + 2 * h * w * O.U * r.dx.abs(), xin.abs())
+        assert O.excess(gw[:, :, 0, 0], dw, dw_tol) <= 0
+        dx = torch.einsum("oi,nohw->nihw", w64, r.dx)
+        dx_tol = torch.einsum("oi,nohw->nihw", w64.abs(), r.dx_tol + cout * O.U * r.dx.abs())
+        assert O.excess(gx, dx, dx_tol) <= 0
+    else:  # against the library's own gradients at the restored input and the block's own gradient of c
+        cc = norm.conv2d(x, blk[0].weight, None).detach().requires_grad_(True)
+        dc, = torch.autograd.grad(norm.group_norm_act(cc, blk[1].num_groups, blk[1].weight, blk[1].bias, blk[1].eps,
+                                                      checkpoint=True), cc, dy)
+        dw = torch.einsum("nohw,nihw->oi", dc.double(), xin)
+        mag = torch.einsum("nohw,nihw->oi", dc.double().abs(), xin.abs())
+        # 2 h w products; an 8-bit value that turns moves its dc by a step: 1 / 64 of its size, in few of them
+        assert O.excess(gw[:, :, 0, 0], dw, (2 * h * w * O.U + 1e-3) * mag) <= 0
+
+
+@gpu
+def test_packed_heads_hold_the_plain_heads_bits():
+    from deep_prob_feature_track_amd import ic
+    dev = _dev()
+    blk = _jitter(convLayer(True, 24, 32, 1, norm="group"), 3).to(dev).to(memory_format=torch.channels_last).eval()
+    x = torch.randn(2, 24, 18, 22, device=dev).contiguous(memory_format=torch.channels_last)
+    with torch.no_grad():
+        conv = blk[0](x)
+        p = blk._group_epilogue(conv, packed=True)
+        assert torch.equal(p, ic.pack_features(blk._group_epilogue(conv)))
+        assert blk.forward_packed(x).shape == (2, 8, 18, 22, 4)
+        nchw = convLayer(True, 24, 32, 1, norm="group").to(dev).eval()
+        assert nchw.forward_packed(x.contiguous()).dim() in (4, 5)
+
+
+@gpu
+def test_encoder_fused_against_modules():
+    """The fused blocks against the torch modules in 64 bits on the CPU, and the packed heads: twenty blocks of
+    at most 3 x 3 x 128 products each, whose roundings (1152 U in the worst order) a block passes on at about
+    their size: 20 x 1152 x 2^-24 of the largest value."""
+    dev = _dev()
+    enc = _encoder(seed=4)
+    x = torch.randn(2, 8, 48, 64, generator=torch.Generator().manual_seed(1))
+    with torch.no_grad():
+        ref = enc.double()(x.double())
+        enc = enc.float().to(dev).to(memory_format=torch.channels_last).eval()
+        xd = x.to(dev).contiguous(memory_format=torch.channels_last)
+        got = enc(xd)
+        packed = enc(xd, packed=True)
+    tol = 20 * 1152 * O.U
+    for a, b in zip(got[0] + got[2], ref[0] + ref[2]):
+        assert (a.cpu().double() - b).abs().max() <= tol * b.abs().max()
+    assert all(p.dim() == 5 for p in packed[0])
+
+
+@gpu
+def test_training_step_keeps_a_quarter():
+    """One step of the encoder: gradients with 8-bit checkpoints beside those without, and the memory that the
+    forward pass holds.  Each stored value is off by at most 1/128 of its block's largest (rms 1/222 of it, and
+    that is about 4 times a value's own rms: 2 % of it); twenty blocks deep, independent: sqrt(20) x 2 % = 9 %,
+    and as much again for the weights' own factors."""
+    dev = _dev()
+    x = torch.randn(2, 8, 96, 128, generator=torch.Generator().manual_seed(2)).to(dev)
+    x = x.contiguous(memory_format=torch.channels_last)
+    grads, held = [], []
+    for ck in (False, True):
+        enc = _encoder(ck, seed=5).to(dev).to(memory_format=torch.channels_last).train()
+        for rep in range(2):  # (the first pass finds the convolutions' algorithms)
+            torch.cuda.synchronize()
+            before = torch.cuda.memory_allocated()
+            f, s, _ = enc(x)
+            loss = sum((t * t).mean() for t in f) + sum(t.log().square().mean() for t in s)
+            outs = sum(t.numel() * t.element_size() for t in f + s)
+            torch.cuda.synchronize()
+            kept = torch.cuda.memory_allocated() - before - outs
+            g = torch.autograd.grad(loss, list(enc.parameters()))
+            del f, s, loss
+        grads.append(g)
+        held.append(kept)
+    for a, b in zip(*grads):
+        assert torch.isfinite(b).all()
+        assert (a - b).norm() <= 0.18 * a.norm() + 1e-6
+    assert held[1] < 0.55 * held[0], held
