@@ -58,7 +58,7 @@ def test_cpu_blocks_run_the_modules():
     blk[0].register_forward_hook(lambda m, i, o: seen.append(o))  # (two runs of a convolution may differ in a bit)
     x = torch.randn(2, 6, 9, 11, requires_grad=True)
     y = blk(x)
-    ref = F.elu(F.group_norm(seen[0], 4, blk[1].weight, blk[1].bias))
+    ref = F.elu(F.group_norm(seen[0], 4, blk[1].weight, blk[1].bias), inplace=True)  # as the module: its gradient
     assert torch.equal(y, ref)
     assert torch.equal(torch.autograd.grad(y.sum(), seen[0], retain_graph=True)[0],
                        torch.autograd.grad(ref.sum(), seen[0])[0])
