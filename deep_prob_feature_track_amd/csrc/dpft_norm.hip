@@ -97,8 +97,8 @@ __device__ __forceinline__ void store_param(void* p, int type, int i, float v) {
 template <typename T>
 __device__ __forceinline__ float expm1_neg(float z) {
   if constexpr (sizeof(T) < 4) {
-    // for a result of 16 bits: to z^3 above -1/16 (the next term is 2^-16.6 of the value there), and
-    // 2^-19.7 below: against half a step of 2^-9 (bf16) or 2^-12 (fp16)
+    // for a result of 16 bits: to z^3 above -1/16 (the next term is at most 2^-16.5 of the value), and
+    // exp(z) - 1 below (2^-19): against half a step of 2^-8 (bf16) or 2^-11 (fp16)
     return z > -0.0625f ? fmaf(z * z, fmaf(z, 1.0f / 6, 0.5f), z) : __expf(z) - 1.0f;
   }
   float q = 1.0f / 720;

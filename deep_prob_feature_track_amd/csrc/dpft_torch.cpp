@@ -77,9 +77,12 @@ DpftGroupNorm check_args(const Tensor& x, int64_t groups, const MaybeTensor& wei
 
 void check_rc(int rc, const char* what) { TORCH_CHECK(rc == DPFT_OK, what, " failed (", rc, "): ", dpft_last_error()); }
 
-// Stored channels_last and 16-byte aligned (a copy where it is not).
+// Stored channels_last (a copy where it is not); and 16-byte aligned (a tensor with memory).
+Tensor ordered(const Tensor& x) {
+  return x.is_contiguous(at::MemoryFormat::ChannelsLast) ? x : x.contiguous(at::MemoryFormat::ChannelsLast);
+}
 Tensor nhwc(const Tensor& x) {
-  Tensor r = x.is_contiguous(at::MemoryFormat::ChannelsLast) ? x : x.contiguous(at::MemoryFormat::ChannelsLast);
+  const Tensor r = ordered(x);
   return reinterpret_cast<uintptr_t>(r.data_ptr()) % 16 ? r.clone(at::MemoryFormat::ChannelsLast) : r;
 }
 Tensor empty_nhwc(const Tensor& x) { return at::empty(x.sizes(), x.options(), at::MemoryFormat::ChannelsLast); }
@@ -199,7 +202,7 @@ struct GroupNormAct : torch::autograd::Function<GroupNormAct> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x0, const MaybeTensor& weight, const MaybeTensor& bias,
                         int64_t groups, double eps, int64_t act, bool checkpoint) {
     at::AutoDispatchBelowADInplaceOrView below;
-    const Tensor x = x0.dim() == 4 && x0.is_cuda() ? nhwc(x0) : x0;  // what is kept is what is read
+    const Tensor x = x0.dim() == 4 && x0.is_cuda() ? ordered(x0) : x0;  // a copy is made once, and kept
     auto [y, stat, q, scale] = forward_op().call(x, groups, weight, bias, eps, act, false, true, checkpoint);
     ctx->save_for_backward({checkpoint ? none(x) : x, q, scale, given(weight) ? *weight : Tensor(),
                             given(bias) ? *bias : Tensor(), stat});

@@ -87,6 +87,9 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="elu", packe
     return _op("group_norm_act")(x, groups, weight, bias, eps, code, packed, checkpoint)
 
 
+_convolution_backward = torch.ops.aten.convolution_backward
+
+
 class _Conv2dCheckpoint(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, stride, padding, dilation, groups):
@@ -103,8 +106,8 @@ class _Conv2dCheckpoint(torch.autograd.Function):
         weight, q, scale = ctx.saved_tensors
         stride, padding, dilation, groups = ctx.conv
         x = act_restore(ActCheckpoint(q, scale, *ctx.layout))
-        dx, dw, db = torch.ops.aten.convolution_backward(dy, x, weight, ctx.bias_sizes, stride, padding, dilation,
-                                                         False, [0, 0], groups, list(ctx.needs_input_grad[:3]))
+        dx, dw, db = _convolution_backward(dy, x, weight, ctx.bias_sizes, stride, padding, dilation, False, [0, 0], groups,
+                                           list(ctx.needs_input_grad[:3]))
         return dx, dw, db, None, None, None, None
 
 

@@ -50,7 +50,9 @@ class Reference:
     The bounds: mean and rstd come from sums of at most `run` terms in a row in fp32 (a thread's) and
     fp64 above that: off by (run + 8) U of the terms' magnitudes.  z takes three roundings more, an
     activation 8 U of its value (its exponential and reciprocal are within 2 U each) and a slope of at
-    most 1.1; a stored value half a step of its type."""
+    most 1.1; a stored value half a step of its type.  The ELU of a 16-bit map is expm1 to z^3 above
+    -1/16: the next term is z^4 / 24 of a value of at least |z| (1 - |z| / 2), so 2^-12 / 24 x 32 / 31 =
+    2^-16.5 of it; below, the exponential's 2 U become at most 2 U x 16 = 2^-19 of the value."""
 
     def __init__(self, x, groups, weight, bias, eps, name, dy=None, checkpoint=False, run=64):
         n, c, h, w = x.shape
@@ -82,7 +84,7 @@ class Reference:
         xhat, xhat_tol, z, z_tol = z_of(x)
         self.z, self.z_tol = z, z_tol
         self.y = act(z, name)
-        y32 = 1.1 * z_tol + 8 * U * self.y.abs()
+        y32 = 1.1 * z_tol + (8 * U + (2.0 ** -16.5 if name == "elu" and t != torch.float32 else 0.0)) * self.y.abs()
         self.y_tol = y32 + half * (self.y.abs() + y32) + tiny
         if dy is None:
             return
