@@ -8,7 +8,11 @@
 // stay in registers.  A row that L cuts short is handled value by value.
 //
 // Everything here moves far more bytes than it computes on (12 to 40 flops per value of 2 to 20
-// bytes): HBM bound at the large sizes, launch bound at the small ones.
+// bytes): HBM bound at the large sizes, launch bound at the small ones.  The figures beside the kernels
+// are of data that no cache holds; a copy of 1 GiB reaches 5.15 TB/s (read and written) on the same card.
+// Two passes over x, not one: kernels that held a sample's values in registers from the statistics to
+// the result, workgroups waiting for each other's sums, took 198 to 303 us where two passes took 213 to
+// 291 -- all of them load, join and store at the same time, and the memory idles in between.
 
 #include <hip/hip_runtime.h>
 
@@ -194,7 +198,7 @@ __device__ __forceinline__ void restore_vec(typename Bytes<V>::type b, float ste
 }
 
 // 16 bytes of x per thread and step, kUnroll steps in flight; the block's maximum by lane shifts.
-// Bound by HBM.
+// Bound by HBM (8 x 32 x 480 x 640 fp32: 63 us, 6.3 TB/s).
 constexpr int kUnroll = 4;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void act_checkpoint_kernel(const T* __restrict__ x, int64_t n,
@@ -232,6 +236,7 @@ __global__ __launch_bounds__(kThreads) void act_checkpoint_kernel(const T* __res
   }
 }
 
+// As the other way (8 x 32 x 480 x 640 fp32, just checkpointed: 56 us, 7.1 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kThreads) void act_restore_kernel(const int8_t* __restrict__ q,
                                                                const uint8_t* __restrict__ scale, int64_t n,
@@ -360,7 +365,8 @@ __device__ __forceinline__ void over_entries(const Walk& w, int tile, int V, int
 // Records [n][parts * tiles][G]: mean, sum of squares about it and count of the workgroup's values of a
 // group.  A thread takes the exact mean of kDeep values of a position, then their squares about it, and
 // joins the batches by the parallel-variance rule; the threads are joined in the same way: nothing
-// cancels, whatever the mean is.
+// cancels, whatever the mean is.  Bound by HBM: 8 x 32 x 480 x 640 fp32 54.7 us, 5.8 TB/s; 16 x 64 x
+// 240 x 320 bf16 31.2 us, 5.0 TB/s.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void gn_stats_kernel(const T* __restrict__ x, Walk w, float4* __restrict__ rec) {
   constexpr int V = Vec<T>::V;
@@ -515,6 +521,8 @@ struct Affine {
 // y = act((x - mean) a + bias), a = rstd * weight.
 // MODE: y as x is stored, in the channel-quad layout, or with x's checkpoint (w.lanes_block).
 // rec: the workgroup joins the statistics itself (kFold groups at most), its part 0 stores them.
+// Bound by HBM: 8 x 32 x 480 x 640 fp32 100.6 us, 6.3 TB/s; 16 x 64 x 240 x 320 bf16 55.4 us, 5.7; with
+// a checkpoint, 8 x 64 x 240 x 320 fp32 65.0 us, 5.5.
 constexpr int kFold = 128;
 enum { kPlain, kPacked, kCheckpoint };
 template <typename T, int ACT, int MODE>
@@ -626,7 +634,9 @@ __global__ __launch_bounds__(kThreads) void gn_apply_kernel(const T* __restrict_
 
 // ------------------------------------------------------------------ small maps
 // A workgroup takes cw channels (whole groups) of a sample and holds all their pixels in registers: one
-// launch, every value read once.  Bound by latency.
+// launch, every value read once.  Bound by latency.  Against two passes, fp32 in a graph: 1 x 128 x 15 x
+// 20 8.1 us (11.5), 32 x 128 x 30 x 34 14.4 (18.2); of one sample only, 8 vectors a thread 9.3 (11.3),
+// 16 vectors 12.6 (11.5).
 constexpr int kSmall = 512;       // threads
 constexpr int kSmallHold = 16;    // vectors of x that a thread holds, in the backward kSmallHold / 2 of x and of dy
 struct Slice {
@@ -844,7 +854,8 @@ struct Coefs {
 };
 
 // With g = dy act'(z): per (sample, part, position of a row) sum g and sum g xhat, and per (sample,
-// part, tile, group) sum weight g and sum weight g xhat.
+// part, tile, group) sum weight g and sum weight g xhat.  Bound by HBM: 16 x 64 x 240 x 320 bf16 52.7 us,
+// 6.0 TB/s; from a checkpoint, 8 x 64 x 240 x 320 fp32 41.8 us, 4.7.
 template <typename T, int ACT, bool Q8>
 __global__ __launch_bounds__(kThreads) void gn_grad_sums_kernel(const T* __restrict__ dy, Source<T, Q8> x, Walk w,
                                                                 Affine f, float2* __restrict__ pos_out,
@@ -1015,7 +1026,8 @@ __global__ __launch_bounds__(kThreads) void gn_param_grads_kernel(Params pg, int
   param_grads(pg.pos, pg.rows, C, type, pg.dweight, pg.dbias, blockIdx.x);
 }
 
-// dx = a g - rstd E[weight g] - (x - mean) rstd^2 E[weight g xhat], a = rstd * weight.
+// dx = a g - rstd E[weight g] - (x - mean) rstd^2 E[weight g xhat], a = rstd * weight.  Bound by HBM:
+// 16 x 64 x 240 x 320 bf16 77.7 us, 6.1 TB/s; from a checkpoint, 8 x 64 x 240 x 320 fp32 58.8 us, 6.0.
 template <typename T, int ACT, bool Q8>
 __global__ __launch_bounds__(kThreads) void gn_grad_input_kernel(const T* __restrict__ dy, Source<T, Q8> x, Walk w,
                                                                  Affine f, Params pg, const float2* __restrict__ rec,
@@ -1209,7 +1221,8 @@ __global__ __launch_bounds__(kSmall) void gn_small_grad_kernel(const T* __restri
 
 // ------------------------------------------------------------------ host side
 // Workgroups of the statistics and of the gradients' sums, whose records the others join, and of those
-// that write.  (Statistics, 8 x 32 x 480 x 640 fp32 in all: 512 168 us, 1024 175, 2048 186.)
+// that write.  (Forward passes in all.  Statistics, 8 x 32 x 480 x 640 fp32: 512 168 us, 1024 175, 2048
+// 186; apply, 8 x 64 x 240 x 320 bf16: 1024 55.7 us, 4096 67.2.)
 constexpr int kStatsWorkgroups = 512, kSumsWorkgroups = 512, kApplyWorkgroups = 1024, kGradWorkgroups = 1024;
 
 int check(const DpftGroupNorm* d) {
@@ -1298,7 +1311,9 @@ size_t need(const DpftGroupNorm& d) {
   return std::max(record_bytes(f, sizeof(float4)) + group_bytes(f),
                   record_bytes(b, sizeof(float2)) + position_bytes(b) + group_bytes(b));
 }
-// The workgroups of the last pass join a sample's records themselves where there are few of them.
+// The workgroups of the last pass join a sample's records themselves where there are few of them: 3 x 30
+// x 61 x 79 bf16, forward and backward 35.1 us, with launches of their own 36.7; 8 x 96 x 120 x 160 fp32
+// 93.1 and 94.3; alike above.  (Each workgroup reads them all: 8192 are 128 KiB.)
 bool fold(const Walk& w) { return w.G <= kFold && (int64_t)w.parts * w.tiles * w.G <= 8192; }
 unsigned waves_grid(int64_t waves) { return (unsigned)((waves + kThreads / 64 - 1) / (kThreads / 64)); }
 unsigned walk_grid(const Walk& w) { return (unsigned)(w.N * w.parts * w.tiles); }
