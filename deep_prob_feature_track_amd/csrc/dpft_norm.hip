@@ -26,7 +26,7 @@
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 256, kWaves = kThreads / 64;
 constexpr int kBlock8 = 32;  // values that share a scale in a checkpoint
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -502,13 +502,15 @@ __device__ __forceinline__ float2 join_stats(const float4* rec, int R, int G, in
 __global__ __launch_bounds__(kThreads) void gn_finish_stats_kernel(const float4* __restrict__ rec, int R, int N, int G,
                                                                    float eps, float* __restrict__ mean,
                                                                    float* __restrict__ rstd) {
-  const int64_t i = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-  if (i >= (int64_t)N * G) return;
-  const int n = (int)(i / G), g = (int)(i - (int64_t)n * G), lane = threadIdx.x & 63;
-  const float2 r = join_stats(rec, R, G, n, g, lane, 64, eps);
-  if (lane == 0) {
-    mean[i] = r.x;
-    rstd[i] = r.y;
+  const int lane = threadIdx.x & 63;
+#pragma unroll 1
+  for (int64_t i = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6); i < (int64_t)N * G; i += (int64_t)gridDim.x * kWaves) {
+    const int n = (int)(i / G), g = (int)(i - (int64_t)n * G);
+    const float2 r = join_stats(rec, R, G, n, g, lane, 64, eps);
+    if (lane == 0) {
+      mean[i] = r.x;
+      rstd[i] = r.y;
+    }
   }
 }
 
@@ -978,11 +980,13 @@ __device__ __forceinline__ float2 join_grads(const float2* rec, int R, const Wal
 }
 __global__ __launch_bounds__(kThreads) void gn_finish_grads_kernel(const float2* __restrict__ rec, int R, Walk w,
                                                                    Affine f, float2* __restrict__ means) {
-  const int64_t i = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
-  if (i >= (int64_t)w.N * w.G) return;
-  const int n = (int)(i / w.G), g = (int)(i - (int64_t)n * w.G), lane = threadIdx.x & 63;
-  const float2 r = join_grads(rec, R, w, f, n, g, lane, 64);
-  if (lane == 0) means[i] = r;
+  const int lane = threadIdx.x & 63;
+#pragma unroll 1
+  for (int64_t i = (int64_t)blockIdx.x * kWaves + (threadIdx.x >> 6); i < (int64_t)w.N * w.G; i += (int64_t)gridDim.x * kWaves) {
+    const int n = (int)(i / w.G), g = (int)(i - (int64_t)n * w.G);
+    const float2 r = join_grads(rec, R, w, f, n, g, lane, 64);
+    if (lane == 0) means[i] = r;
+  }
 }
 
 // dweight and dbias from `rows` rows of (sum g, sum g xhat) per channel: 8 channels a workgroup, the
@@ -1315,7 +1319,7 @@ size_t need(const DpftGroupNorm& d) {
 // x 61 x 79 bf16, forward and backward 35.1 us, with launches of their own 36.7; 8 x 96 x 120 x 160 fp32
 // 93.1 and 94.3; alike above.  (Each workgroup reads them all: 8192 are 128 KiB.)
 bool fold(const Walk& w) { return w.G <= kFold && (int64_t)w.parts * w.tiles * w.G <= 8192; }
-unsigned waves_grid(int64_t waves) { return (unsigned)((waves + kThreads / 64 - 1) / (kThreads / 64)); }
+unsigned waves_grid(int64_t waves) { return (unsigned)std::min<int64_t>((waves + kWaves - 1) / kWaves, int64_t(1) << 20); }
 unsigned walk_grid(const Walk& w) { return (unsigned)(w.N * w.parts * w.tiles); }
 bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
 

@@ -33,10 +33,13 @@ int32_t type_code(at::ScalarType t, const char* what) {
   return DPFT_TYPE_F16;
 }
 
-void check_param(const MaybeTensor& p, const char* name, const Tensor& x) {
+// A traced call's channels are what it was traced with; its batch and pixels may be symbols.
+int64_t channels(const Tensor& t, int64_t dim) { return t.sym_size(dim).guard_int(__FILE__, __LINE__); }
+
+void check_param(const MaybeTensor& p, const char* name, const Tensor& x, int64_t C) {
   if (!p || !p->defined()) return;
-  TORCH_CHECK_VALUE(p->dim() == 1 && p->size(0) == x.size(1), name, " must hold one value per channel (", x.size(1),
-                    "), got ", p->sizes());
+  TORCH_CHECK_VALUE(p->dim() == 1 && channels(*p, 0) == C, name, " must hold one value per channel (", C, "), got ",
+                    p->sym_sizes());
   type_code(p->scalar_type(), name);
   TORCH_CHECK_VALUE(p->device() == x.device(), name, " is on ", p->device(), ", expected ", x.device());
 }
@@ -45,24 +48,22 @@ bool given(const MaybeTensor& t) { return t && t->defined(); }
 void* ptr(const MaybeTensor& t) { return given(t) && t->numel() ? t->data_ptr() : nullptr; }
 Tensor dense(const MaybeTensor& t) { return given(t) ? t->contiguous() : Tensor(); }
 
-// Everything that the arguments have to meet, on any device.
+// Everything that the arguments have to meet, on any device and in a trace.
 DpftGroupNorm check_args(const Tensor& x, int64_t groups, const MaybeTensor& weight, const MaybeTensor& bias, double eps,
                          int64_t act, bool packed) {
-  TORCH_CHECK_VALUE(x.dim() == 4, "group_norm_act needs a map [N,C,H,W], got ", x.sizes());
-  const int64_t C = x.size(1);
+  TORCH_CHECK_VALUE(x.dim() == 4, "group_norm_act needs a map [N,C,H,W], got ", x.sym_sizes());
+  const int64_t C = channels(x, 1);
   TORCH_CHECK_VALUE(groups >= 1 && C >= 1 && C % groups == 0, "groups=", groups, " does not divide C=", C);
   TORCH_CHECK_VALUE(eps >= 0, "eps must not be negative (got ", eps, ")");
-  check_param(weight, "weight", x);
-  check_param(bias, "bias", x);
+  check_param(weight, "weight", x, C);
+  check_param(bias, "bias", x, C);
   if (given(weight) && given(bias))
     TORCH_CHECK_TYPE(weight->scalar_type() == bias->scalar_type(), "weight and bias must have one dtype (got ",
                      weight->scalar_type(), ", ", bias->scalar_type(), ")");
   TORCH_CHECK_VALUE(!packed || (x.scalar_type() == at::kFloat && C % 4 == 0), "packed=True needs fp32 and C % 4 == 0, got ",
-                    x.scalar_type(), " ", x.sizes());
-  TORCH_CHECK_VALUE(x.size(0) <= INT32_MAX && C <= INT32_MAX, "too large: ", x.sizes());
+                    x.scalar_type(), " ", x.sym_sizes());
+  TORCH_CHECK_VALUE(C <= INT32_MAX, "too large: ", x.sym_sizes());
   DpftGroupNorm d{};
-  d.pixels = x.size(2) * x.size(3);
-  d.N = (int32_t)x.size(0);
   d.C = (int32_t)C;
   d.groups = (int32_t)groups;
   d.act = (int32_t)act;
@@ -72,6 +73,14 @@ DpftGroupNorm check_args(const Tensor& x, int64_t groups, const MaybeTensor& wei
                                : DPFT_TYPE_F32;
   d.flags = packed ? DPFT_GN_PACKED : 0;
   d.eps = (float)eps;
+  return d;
+}
+
+// ... and the sizes of a map with memory.
+DpftGroupNorm sized(DpftGroupNorm d, const Tensor& x) {
+  TORCH_CHECK_VALUE(x.size(0) <= INT32_MAX, "too large: ", x.sizes());
+  d.pixels = x.size(2) * x.size(3);
+  d.N = (int32_t)x.size(0);
   return d;
 }
 
@@ -113,7 +122,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> forward_outputs(const Tensor& x, int6
 std::tuple<Tensor, Tensor, Tensor, Tensor> forward_hip(const Tensor& x0, int64_t groups, const MaybeTensor& weight,
                                                        const MaybeTensor& bias, double eps, int64_t act, bool packed,
                                                        bool stats, bool checkpoint) {
-  const DpftGroupNorm d = check_args(x0, groups, weight, bias, eps, act, packed);
+  const DpftGroupNorm d = sized(check_args(x0, groups, weight, bias, eps, act, packed), x0);
   const c10::DeviceGuard guard(x0.device());
   const Tensor x = nhwc(x0), w = dense(weight), b = dense(bias);
   auto out = forward_outputs(x, groups, packed, stats, checkpoint);
@@ -131,7 +140,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> forward_meta(const Tensor& x, int64_t
                                                         const MaybeTensor& bias, double eps, int64_t act, bool packed,
                                                         bool stats, bool checkpoint) {
   check_args(x, groups, weight, bias, eps, act, packed);
-  return forward_outputs(x, groups, packed, stats, checkpoint);
+  const auto N = x.sym_size(0), C = x.sym_size(1), H = x.sym_size(2), W = x.sym_size(3), n = x.sym_numel();
+  Tensor y = packed ? at::empty_symint({N, C / 4, H, W, 4}, x.options())
+                    : at::empty_symint({N, C, H, W}, x.options(), at::MemoryFormat::ChannelsLast);
+  Tensor stat = stats ? at::empty_symint({2, N, groups}, x.options().dtype(at::kFloat)) : none(x);
+  Tensor q = checkpoint ? at::empty_symint({n}, x.options().dtype(at::kChar)) : none(x);
+  Tensor scale = checkpoint ? at::empty_symint({(n + kBlock8 - 1) / kBlock8}, x.options().dtype(at::kByte)) : none(x);
+  return {y, stat, q, scale};
 }
 std::tuple<Tensor, Tensor, Tensor, Tensor> forward_cpu(const Tensor& x, int64_t groups, const MaybeTensor& weight,
                                                        const MaybeTensor& bias, double eps, int64_t act, bool packed,
@@ -151,7 +166,7 @@ std::tuple<Tensor, Tensor, Tensor> backward_hip(const Tensor& dy0, const Tensor&
                                                 const MaybeTensor& weight, const MaybeTensor& bias, const Tensor& stat,
                                                 int64_t groups, double eps, int64_t act, bool need_x, bool need_w,
                                                 bool need_b) {
-  const DpftGroupNorm d = check_args(dy0, groups, weight, bias, eps, act, false);
+  const DpftGroupNorm d = sized(check_args(dy0, groups, weight, bias, eps, act, false), dy0);
   const int64_t n = dy0.numel();
   const bool from_x = x.numel() != 0 && q.numel() == 0 && x.sizes() == dy0.sizes() && x.scalar_type() == dy0.scalar_type(),
              from_q = x.numel() == 0 && q.numel() == n && scale.numel() == blocks_of(n) && q.is_contiguous() &&
@@ -182,7 +197,8 @@ std::tuple<Tensor, Tensor, Tensor> backward_hip(const Tensor& dy0, const Tensor&
 std::tuple<Tensor, Tensor, Tensor> backward_meta(const Tensor& dy, const Tensor&, const Tensor&, const Tensor&,
                                                  const MaybeTensor& weight, const MaybeTensor& bias, const Tensor&, int64_t,
                                                  double, int64_t, bool need_x, bool need_w, bool need_b) {
-  return backward_outputs(dy, weight, bias, need_x, need_w, need_b);
+  return {need_x ? at::empty_symint(dy.sym_sizes(), dy.options(), at::MemoryFormat::ChannelsLast) : none(dy),
+          need_w ? at::empty_like(*weight) : none(dy), need_b ? at::empty_like(*bias) : none(dy)};
 }
 
 auto& forward_op() {

@@ -13,6 +13,7 @@ import torch
 import torch.nn as nn
 from torch.nn import init
 
+from .. import _native as N
 from .. import ic
 from .. import norm as gn
 from .. import torch_ops  # noqa: F401  (registers the dpft:: ops torch.compile traces)
@@ -54,18 +55,19 @@ class ConvBlock(nn.Sequential):
     act_checkpoint = False
 
     def _group(self, x):
-        return (len(self) == 3 and isinstance(self[0], nn.Conv2d) and isinstance(self[1], nn.GroupNorm)
-                and isinstance(self[2], nn.ELU) and self[2].alpha == 1.0 and x.is_cuda)
+        return (len(self) == 3 and isinstance(self[0], nn.Conv2d) and type(self[1]) is nn.GroupNorm
+                and type(self[2]) is nn.ELU and self[2].alpha == 1.0 and x.is_cuda)
 
     def _group_conv(self, x):
         c = self[0]
-        if self.act_checkpoint and torch.is_grad_enabled() and c.padding_mode == 'zeros':
+        if (self.act_checkpoint and torch.is_grad_enabled() and type(c) is nn.Conv2d and c.padding_mode == 'zeros'
+                and not isinstance(c.padding, str) and x.dim() == 4 and x.dtype in N.TYPES):
             return gn.conv2d(x, c.weight, c.bias, c.stride, c.padding, c.dilation, c.groups)
         return c(x)
 
     def _group_epilogue(self, y, packed=False):
         n = self[1]
-        if not y.is_contiguous(memory_format=torch.channels_last):
+        if y.dim() != 4 or y.dtype not in N.TYPES or not y.is_contiguous(memory_format=torch.channels_last):
             return self[2](n(y))
         return gn.group_norm_act(y, n.num_groups, n.weight, n.bias, n.eps, "elu", packed=packed,
                                  checkpoint=self.act_checkpoint)
@@ -81,8 +83,7 @@ class ConvBlock(nn.Sequential):
         [B,C,H,W].  Same values either way."""
         if self._group(x) and not torch.is_grad_enabled():
             y = self[0](x)
-            return self._group_epilogue(y, packed=y.dtype == torch.float32 and y.shape[1] % 4 == 0 and y.is_contiguous(
-                memory_format=torch.channels_last))
+            return self._group_epilogue(y, packed=y.dtype == torch.float32 and y.dim() == 4 and y.shape[1] % 4 == 0)
         if self._fusable(x):
             y = self[0](x)
             if ic.bn_elu_pack_applies(y, self[1]):

@@ -123,6 +123,8 @@ def conv2d(x, weight, bias=None, stride=1, padding=0, dilation=1, groups=1):
         raise ValueError(f"padding must be numbers (got {padding!r})")
     if not x.is_cuda:
         raise RuntimeError("conv2d needs a device tensor; there is no CPU fallback")
+    if x.dim() != 4:
+        raise ValueError(f"conv2d needs a map [N,C,H,W], got {tuple(x.shape)}")
     args = (_pair(stride), _pair(padding), _pair(dilation), groups)
     if not (torch.is_grad_enabled() and weight.requires_grad):  # the backward pass does not read x
         return torch.nn.functional.conv2d(x, weight, bias, *args)

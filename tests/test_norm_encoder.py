@@ -204,6 +204,8 @@ def test_packed_heads_hold_the_plain_heads_bits():
         p = blk._group_epilogue(conv, packed=True)
         assert torch.equal(p, ic.pack_features(blk._group_epilogue(conv)))
         assert blk.forward_packed(x).shape == (2, 8, 18, 22, 4)
+        wide = conv.double()  # (a type that the kernels do not have: the modules)
+        assert torch.equal(blk.double()._group_epilogue(wide.clone(memory_format=torch.channels_last)), blk[2](blk[1](wide)))
         nchw = convLayer(True, 24, 32, 1, norm="group").to(dev).eval()
         assert nchw.forward_packed(x.contiguous()).dim() in (4, 5)
 

@@ -110,11 +110,33 @@ def test_entry_points_refuse_without_device_work():
         assert f(3, 8, p) == f(0, 0, p) == f(0, 8, None) == f(0, 8, ctypes.c_void_p(4097)) == f(0, 1 << 60, p) == -1
 
 
+@pytest.mark.parametrize("checkpoint", [False, True])
+def test_traces_with_symbolic_sizes(checkpoint):
+    """Forward and backward in a trace whose batch and pixels are symbols: the operators, shapes and layouts."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    def step(x, w, b):
+        y = norm.group_norm_act(x, 4, w, b, checkpoint=checkpoint)
+        return (y,) + torch.autograd.grad(y, (x, w, b), torch.ones_like(y))
+    x = _map(2, 8, 6, 10, F32).requires_grad_(True)
+    w, b = (p.requires_grad_(True) for p in _params(8))
+    g = make_fx(step, tracing_mode="symbolic", _allow_non_fake_inputs=True)(x, w, b)
+    names = [n.target.__name__ for n in g.graph.nodes if n.op == "call_function"]
+    assert names.count("group_norm_act_forward.default") == names.count("group_norm_act_backward.default") == 1
+    out = [n for n in g.graph.nodes if n.op == "output"][0].args[0]
+    y, dx, dw, db = (n.meta["val"] for n in out)
+    assert not isinstance(y.shape[2], int)  # a symbol
+    assert y.stride(1) == dx.stride(1) == 1 and y.dtype == F32 and dw.shape == db.shape == (8,)
+    p = make_fx(lambda t: norm.group_norm_act(t, 4, packed=True), tracing_mode="symbolic")(x.detach())
+    assert [n for n in p.graph.nodes if n.op == "output"][0].args[0].meta["val"].dim() == 5
+
+
 # ------------------------------------------------------------------ the kernels
 SHAPES = [  # N, C, H, W, groups
     (1, 1, 1, 1, 1), (2, 6, 1, 1, 3), (1, 8, 5, 7, 2), (3, 30, 9, 11, 5), (2, 13, 17, 5, 1), (1, 7, 3, 50, 7),
     (1, 32, 64, 80, 8), (2, 96, 15, 20, 8), (16, 16, 9, 9, 4), (1, 300, 7, 3, 4), (1, 257, 3, 5, 1),
-    (2, 1030, 2, 3, 5), (1, 2056, 1, 3, 8), (5, 64, 33, 1, 64), (1, 4, 300, 301, 1)]
+    (2, 1030, 2, 3, 5), (1, 2056, 1, 3, 8), (5, 64, 33, 1, 64), (1, 4, 300, 301, 1),
+    (2, 258, 5, 6, 129), (1, 400, 9, 7, 200)]  # (groups of a launch of their own)
 
 
 def _check(r, y=None, dx=None, dw=None, db=None, p_half=O.U):
@@ -417,6 +439,8 @@ def test_conv2d_gives_the_restored_input(cl, autocast, monkeypatch):
     assert a == ([12], [2, 2], [1, 2], [2, 2], False, [0, 0], 2, [True, True, True])
     assert (dx == 1).all() and (dw == 2).all() and (db == 3).all()
     assert dx.dtype == dw.dtype == db.dtype == F32  # the leaves' own
+    with pytest.raises(ValueError):
+        norm.conv2d(x[0], wt, b, 2, (1, 2), dilation=2, groups=2)
     del given[:]
     z = norm.conv2d(x, wt.detach(), b, 2, (1, 2), dilation=2, groups=2)  # no gradient of the weight: nothing kept
     assert z.requires_grad and "Checkpoint" not in type(z.grad_fn).__name__ and not given
@@ -439,6 +463,9 @@ def test_compiled_call_is_the_eager_one():
         assert torch.equal(y, z)
         for u, v in zip(_grads(y, (x, wt, b), dy), _grads(z, (x, wt, b), dy)):
             assert torch.equal(u, v)
+        for h, w in ((7, 20), (5, 4)):  # other sizes, which then are symbols
+            x = _map(3, 16, h, w, F32, dev=dev).requires_grad_(True)
+            assert torch.equal(block(x, ck), fast(x, ck))
 
 
 @gpu
@@ -513,6 +540,34 @@ def test_runs_are_bit_identical_and_streams_share_nothing():
     torch.cuda.synchronize()
     for a, r in zip(outs, ref):
         assert all(torch.equal(u, v) for u, v in zip(a, r))
+
+
+@gpu
+def test_two_threads_at_once():
+    """Calls from two host threads, each on a stream of its own, and in inference mode."""
+    import threading
+    dev = _dev()
+    wt, b = _params(24, dev=dev)
+    xs = [_map(2, 24, 40, 50, F32, seed=i, dev=dev) for i in range(2)]
+    ref = [norm.group_norm_act(x, 6, wt, b) for x in xs]
+    with torch.inference_mode():
+        assert torch.equal(norm.group_norm_act(xs[0], 6, wt, b), ref[0])
+    torch.cuda.synchronize()
+    got = [[], []]
+
+    def work(i):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got[i].append(norm.group_norm_act(xs[i], 6, wt, b))
+        s.synchronize()
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert all(len(g) == 20 and all(torch.equal(y, r) for y in g) for g, r in zip(got, ref))
 
 
 @gpu
