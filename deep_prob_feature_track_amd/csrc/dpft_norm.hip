@@ -97,25 +97,31 @@ __device__ __forceinline__ void store_param(void* p, int type, int i, float v) {
 
 // ------------------------------------------------------------------ activations
 // expm1 on z <= 0: its Taylor polynomial to z^6 above -1/4 (the next term is 4.8e-8 of the value
-// there), exp(z) - 1 below (whose error of 1.2 x 2^-24 is at most 5.5 x 2^-24 of the value).
+// there), exp(z) - 1 below (whose error of 1.2 x 2^-24 is at most 5.5 x 2^-24 of the value).  Both are
+// computed and one is selected: as branches, which lanes part at, a value after the other.
 template <typename T>
 __device__ __forceinline__ float expm1_neg(float z) {
   if constexpr (sizeof(T) < 4) {
     // for a result of 16 bits: to z^3 above -1/16 (the next term is at most 2^-16.5 of the value), and
     // exp(z) - 1 below (2^-19): against half a step of 2^-8 (bf16) or 2^-11 (fp16)
-    return z > -0.0625f ? fmaf(z * z, fmaf(z, 1.0f / 6, 0.5f), z) : __expf(z) - 1.0f;
+    const float near = fmaf(z * z, fmaf(z, 1.0f / 6, 0.5f), z), far = __expf(z) - 1.0f;
+    return z > -0.0625f ? near : far;
   }
   float q = 1.0f / 720;
   q = fmaf(q, z, 1.0f / 120);
   q = fmaf(q, z, 1.0f / 24);
   q = fmaf(q, z, 1.0f / 6);
   q = fmaf(q, z, 0.5f);
-  return z > -0.25f ? fmaf(z * z, q, z) : __expf(z) - 1.0f;
+  const float near = fmaf(z * z, q, z), far = __expf(z) - 1.0f;
+  return z > -0.25f ? near : far;
 }
 template <int ACT, typename T>
 __device__ __forceinline__ float act_fwd(float z) {
   if constexpr (ACT == DPFT_ACT_RELU) return z < 0.0f ? 0.0f : z;
-  if constexpr (ACT == DPFT_ACT_ELU) return z > 0.0f ? z : expm1_neg<T>(z);
+  if constexpr (ACT == DPFT_ACT_ELU) {
+    const float below = expm1_neg<T>(z);
+    return z > 0.0f ? z : below;
+  }
   if constexpr (ACT == DPFT_ACT_SILU) return z * __builtin_amdgcn_rcpf(1.0f + __expf(-z));
   return z;
 }
@@ -317,9 +323,13 @@ struct Block {
   __device__ __forceinline__ Block(const Walk& w, const Place& p, int b, int deep, int V) {
     const int64_t r0 = (int64_t)b * deep * w.RS;
     at = p.n * w.L + r0 * w.Cv;
-    whole = (int)min((w.full - r0) / w.RS, (int64_t)deep);
-    const int64_t r = r0 + (int64_t)whole * w.RS + p.rr;
-    tail = whole == deep ? 0 : r < w.full ? V : r == w.full ? tail_values(w, p.slot, V) : 0;
+    whole = deep;
+    tail = 0;
+    if (b == w.blocks - 1) {  // (the others are whole: the division stays out of the loops)
+      whole = (int)min((w.full - r0) / w.RS, (int64_t)deep);
+      const int64_t r = r0 + (int64_t)whole * w.RS + p.rr;
+      tail = whole == deep ? 0 : r < w.full ? V : r == w.full ? tail_values(w, p.slot, V) : 0;
+    }
   }
   // Values of the cut row that fall to `slot`.
   static __device__ __forceinline__ int tail_values(const Walk& w, int slot, int V) {
@@ -1226,8 +1236,9 @@ __global__ __launch_bounds__(kSmall) void gn_small_grad_kernel(const T* __restri
 // ------------------------------------------------------------------ host side
 // Workgroups of the statistics and of the gradients' sums, whose records the others join, and of those
 // that write.  (Forward passes in all.  Statistics, 8 x 32 x 480 x 640 fp32: 512 168 us, 1024 175, 2048
-// 186; apply, 8 x 64 x 240 x 320 bf16: 1024 55.7 us, 4096 67.2.)
-constexpr int kStatsWorkgroups = 512, kSumsWorkgroups = 512, kApplyWorkgroups = 1024, kGradWorkgroups = 1024;
+// 186; apply, 8 x 64 x 240 x 320 bf16: 1024 55.7 us, 4096 67.2.  Both that write, forward and backward, 16 x
+// 64 x 240 x 320 bf16: 1024 228.7 us, 1280 224.8, which all fit at once.)
+constexpr int kStatsWorkgroups = 512, kSumsWorkgroups = 512, kApplyWorkgroups = 1280, kGradWorkgroups = 1280;
 
 int check(const DpftGroupNorm* d) {
   if (!d) return dpft_fail(DPFT_E_INVALID, "null descriptor");
