@@ -1240,6 +1240,11 @@ __global__ __launch_bounds__(kSmall) void gn_small_grad_kernel(const T* __restri
 // 64 x 240 x 320 bf16: 1024 228.7 us, 1280 224.8, which all fit at once.)
 constexpr int kStatsWorkgroups = 512, kSumsWorkgroups = 512, kApplyWorkgroups = 1280, kGradWorkgroups = 1280;
 
+// Slots of a tile where the result is in the channel-quad layout, in which a slot's pixels lie side by side and
+// slots a plane apart: 32 pixels a workgroup, 512 bytes in a row (3 x 512 x 62 x 314: a whole row's 128 slots
+// and 2 pixels 356 us, 16 slots 90, 8 slots 85; 8 x 32 x 240 x 320, of 8 slots, 47 either way).
+constexpr int kPackedSlots = 8;
+
 int check(const DpftGroupNorm* d) {
   if (!d) return dpft_fail(DPFT_E_INVALID, "null descriptor");
   if (d->N < 1 || d->C < 1 || d->pixels < 1 || d->groups < 1)
@@ -1260,8 +1265,8 @@ int check(const DpftGroupNorm* d) {
   return DPFT_OK;
 }
 
-// deep: vectors that a thread visits in a block.
-Walk make_walk(const DpftGroupNorm& d, int deep, int workgroups) {
+// deep: vectors that a thread visits in a block; slots: of a tile at most.
+Walk make_walk(const DpftGroupNorm& d, int deep, int workgroups, int slots = kThreads) {
   Walk w{};
   const int V = d.x_type == DPFT_TYPE_F32 ? 4 : 8;
   w.N = d.N;
@@ -1271,8 +1276,8 @@ Walk make_walk(const DpftGroupNorm& d, int deep, int workgroups) {
   w.L = d.pixels * d.C;
   w.Cv = std::lcm(d.C, V);
   w.S = w.Cv / V;
-  w.W = std::min(w.S, kThreads);
-  w.tiles = (w.S + w.W - 1) / w.W;
+  w.tiles = (w.S + slots - 1) / slots;
+  w.W = (w.S + w.tiles - 1) / w.tiles;
   w.RS = kThreads / w.W;
   const int whole = kBlock8 / std::gcd(w.Cv, kBlock8);  // rows that make whole checkpoint blocks
   if (w.RS >= whole) w.RS -= w.RS % whole;
@@ -1328,8 +1333,9 @@ size_t need(const DpftGroupNorm& d) {
 }
 // The workgroups of the last pass join a sample's records themselves where there are few of them: 3 x 30
 // x 61 x 79 bf16, forward and backward 35.1 us, with launches of their own 36.7; 8 x 96 x 120 x 160 fp32
-// 93.1 and 94.3; alike above.  (Each workgroup reads them all: 8192 are 128 KiB.)
-bool fold(const Walk& w) { return w.G <= kFold && (int64_t)w.parts * w.tiles * w.G <= 8192; }
+// 93.1 and 94.3.  Each workgroup reads them all, 16 KiB for 1024: one sample of 384 x 16 x 636 fp16 in 16
+// groups took 63.7 us with up to 8192, 52.9 so.
+bool fold(const Walk& w) { return w.G <= kFold && (int64_t)w.parts * w.tiles * w.G <= 1024; }
 unsigned waves_grid(int64_t waves) { return (unsigned)std::min<int64_t>((waves + kWaves - 1) / kWaves, int64_t(1) << 20); }
 unsigned walk_grid(const Walk& w) { return (unsigned)(w.N * w.parts * w.tiles); }
 bool misaligned(const void* p) { return reinterpret_cast<uintptr_t>(p) & 15; }
@@ -1343,7 +1349,8 @@ void launch_forward(const DpftGroupNorm& d, const T* x, Affine f, float* mean_ou
                        d.eps, mean_out, rstd_out, y, q, scale);
     return;
   }
-  const Walk ws1 = make_walk(d, kDeep, kStatsWorkgroups), w = make_walk(d, kDeepApply, kApplyWorkgroups);
+  const Walk ws1 = make_walk(d, kDeep, kStatsWorkgroups),
+             w = make_walk(d, kDeepApply, kApplyWorkgroups, MODE == kPacked ? kPackedSlots : kThreads);
   const int R = ws1.parts * ws1.tiles;
   const dim3 block(kThreads);
   float4* rec = static_cast<float4*>(ws);
