@@ -204,7 +204,7 @@ __device__ __forceinline__ void restore_vec(typename Bytes<V>::type b, float ste
 }
 
 // 16 bytes of x per thread and step, kUnroll steps in flight; the block's maximum by lane shifts.
-// Bound by HBM (8 x 32 x 480 x 640 fp32: 63 us, 6.3 TB/s).
+// Bound by HBM (8 x 32 x 480 x 640 fp32: 64 us, 6.2 TB/s).
 constexpr int kUnroll = 4;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void act_checkpoint_kernel(const T* __restrict__ x, int64_t n,
@@ -375,8 +375,8 @@ __device__ __forceinline__ void over_entries(const Walk& w, int tile, int V, int
 // Records [n][parts * tiles][G]: mean, sum of squares about it and count of the workgroup's values of a
 // group.  A thread takes the exact mean of kDeep values of a position, then their squares about it, and
 // joins the batches by the parallel-variance rule; the threads are joined in the same way: nothing
-// cancels, whatever the mean is.  Bound by HBM: 8 x 32 x 480 x 640 fp32 54.7 us, 5.8 TB/s; 16 x 64 x
-// 240 x 320 bf16 31.2 us, 5.0 TB/s.
+// cancels, whatever the mean is.  Bound by HBM: 8 x 32 x 480 x 640 fp32 53.0 us, 5.9 TB/s; 16 x 64 x
+// 240 x 320 bf16 30.7 us, 5.1 TB/s.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void gn_stats_kernel(const T* __restrict__ x, Walk w, float4* __restrict__ rec) {
   constexpr int V = Vec<T>::V;
@@ -533,8 +533,8 @@ struct Affine {
 // y = act((x - mean) a + bias), a = rstd * weight.
 // MODE: y as x is stored, in the channel-quad layout, or with x's checkpoint (w.lanes_block).
 // rec: the workgroup joins the statistics itself (kFold groups at most), its part 0 stores them.
-// Bound by HBM: 8 x 32 x 480 x 640 fp32 100.6 us, 6.3 TB/s; 16 x 64 x 240 x 320 bf16 55.4 us, 5.7; with
-// a checkpoint, 8 x 64 x 240 x 320 fp32 65.0 us, 5.5.
+// Bound by HBM: 8 x 32 x 480 x 640 fp32 100.6 us, 6.3 TB/s; 16 x 64 x 240 x 320 bf16 52.9 us, 5.9; with
+// a checkpoint, 8 x 64 x 240 x 320 fp32 64.4 us, 5.5.
 constexpr int kFold = 128;
 enum { kPlain, kPacked, kCheckpoint };
 template <typename T, int ACT, int MODE>
@@ -866,8 +866,8 @@ struct Coefs {
 };
 
 // With g = dy act'(z): per (sample, part, position of a row) sum g and sum g xhat, and per (sample,
-// part, tile, group) sum weight g and sum weight g xhat.  Bound by HBM: 16 x 64 x 240 x 320 bf16 52.7 us,
-// 6.0 TB/s; from a checkpoint, 8 x 64 x 240 x 320 fp32 41.8 us, 4.7.
+// part, tile, group) sum weight g and sum weight g xhat.  Bound by HBM: 16 x 64 x 240 x 320 bf16 53.6 us,
+// 5.9 TB/s; from a checkpoint, 8 x 64 x 240 x 320 fp32 41.2 us, 4.8.
 template <typename T, int ACT, bool Q8>
 __global__ __launch_bounds__(kThreads) void gn_grad_sums_kernel(const T* __restrict__ dy, Source<T, Q8> x, Walk w,
                                                                 Affine f, float2* __restrict__ pos_out,
@@ -1041,7 +1041,7 @@ __global__ __launch_bounds__(kThreads) void gn_param_grads_kernel(Params pg, int
 }
 
 // dx = a g - rstd E[weight g] - (x - mean) rstd^2 E[weight g xhat], a = rstd * weight.  Bound by HBM:
-// 16 x 64 x 240 x 320 bf16 77.7 us, 6.1 TB/s; from a checkpoint, 8 x 64 x 240 x 320 fp32 58.8 us, 6.0.
+// 16 x 64 x 240 x 320 bf16 79.6 us, 5.9 TB/s; from a checkpoint, 8 x 64 x 240 x 320 fp32 59.8 us, 5.9.
 template <typename T, int ACT, bool Q8>
 __global__ __launch_bounds__(kThreads) void gn_grad_input_kernel(const T* __restrict__ dy, Source<T, Q8> x, Walk w,
                                                                  Affine f, Params pg, const float2* __restrict__ rec,

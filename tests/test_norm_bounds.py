@@ -12,7 +12,8 @@ CLANG = os.path.join(B.LLVM_BIN, "clang++")
 SIZES = [  # N, C, H, W, groups
     (1, 1, 1, 1, 1), (2, 6, 1, 1, 3), (1, 8, 5, 7, 2), (2, 13, 17, 5, 1), (2, 20, 9, 11, 4), (3, 30, 9, 11, 5), (1, 7, 3, 50, 7),
     (2, 96, 15, 20, 8), (2, 32, 33, 32, 8), (1, 257, 3, 5, 1), (2, 1030, 2, 3, 5), (1, 2056, 1, 3, 8), (2, 258, 5, 6, 129),
-    (1, 400, 9, 7, 200), (1, 4, 100, 101, 1), (2, 128, 6, 8, 8)]
+    (1, 400, 9, 7, 200), (1, 4, 100, 101, 1), (2, 128, 6, 8, 8), (1, 36, 20, 21, 3),
+    (1, 260, 5, 7, 5)]
 
 
 @pytest.fixture(scope="module")

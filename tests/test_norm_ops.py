@@ -187,7 +187,7 @@ def test_relu(dtype):
 
 
 @gpu
-@pytest.mark.parametrize("c,h,w", [(32, 24, 40), (4, 3, 5), (20, 7, 9)])
+@pytest.mark.parametrize("c,h,w", [(32, 24, 40), (4, 3, 5), (20, 7, 9), (36, 40, 41), (512, 30, 21)])
 def test_packed_layout(c, h, w):
     """The channel-quad output holds the plain output's bits."""
     from deep_prob_feature_track_amd import ic
