@@ -45,12 +45,26 @@ void check_param(const MaybeTensor& p, const char* name, const Tensor& x, int64_
 }
 
 bool given(const MaybeTensor& t) { return t && t->defined(); }
+
+// The operators have no forward-mode derivative.  A tangent would be lost without a word below autograd, whether or
+// not anything requires a gradient: every way in asks for it.
+void refuse_tangents(std::initializer_list<const Tensor*> inputs) {
+  for (const Tensor* t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(),
+                                "group_norm_act has no forward-mode derivative (an input carries a tangent)");
+}
+void refuse_tangents(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias) {
+  refuse_tangents({&x});
+  if (weight) refuse_tangents({&*weight});
+  if (bias) refuse_tangents({&*bias});
+}
 void* ptr(const MaybeTensor& t) { return given(t) && t->numel() ? t->data_ptr() : nullptr; }
 Tensor dense(const MaybeTensor& t) { return given(t) ? t->contiguous() : Tensor(); }
 
 // Everything that the arguments have to meet, on any device and in a trace.
 DpftGroupNorm check_args(const Tensor& x, int64_t groups, const MaybeTensor& weight, const MaybeTensor& bias, double eps,
                          int64_t act, bool packed) {
+  refuse_tangents(x, weight, bias);
   TORCH_CHECK_VALUE(x.dim() == 4, "group_norm_act needs a map [N,C,H,W], got ", x.sym_sizes());
   const int64_t C = channels(x, 1);
   TORCH_CHECK_VALUE(groups >= 1 && C >= 1 && C % groups == 0, "groups=", groups, " does not divide C=", C);
@@ -166,6 +180,7 @@ std::tuple<Tensor, Tensor, Tensor> backward_hip(const Tensor& dy0, const Tensor&
                                                 const MaybeTensor& weight, const MaybeTensor& bias, const Tensor& stat,
                                                 int64_t groups, double eps, int64_t act, bool need_x, bool need_w,
                                                 bool need_b) {
+  refuse_tangents({&x});
   const DpftGroupNorm d = sized(check_args(dy0, groups, weight, bias, eps, act, false), dy0);
   const int64_t n = dy0.numel();
   const bool from_x = x.numel() != 0 && q.numel() == 0 && x.sizes() == dy0.sizes() && x.scalar_type() == dy0.scalar_type(),
@@ -194,9 +209,11 @@ std::tuple<Tensor, Tensor, Tensor> backward_hip(const Tensor& dy0, const Tensor&
            "dpft_group_norm_act_backward");
   return out;
 }
-std::tuple<Tensor, Tensor, Tensor> backward_meta(const Tensor& dy, const Tensor&, const Tensor&, const Tensor&,
+std::tuple<Tensor, Tensor, Tensor> backward_meta(const Tensor& dy, const Tensor& x, const Tensor&, const Tensor&,
                                                  const MaybeTensor& weight, const MaybeTensor& bias, const Tensor&, int64_t,
                                                  double, int64_t, bool need_x, bool need_w, bool need_b) {
+  refuse_tangents({&x});
+  refuse_tangents(dy, weight, bias);
   return {need_x ? at::empty_symint(dy.sym_sizes(), dy.options(), at::MemoryFormat::ChannelsLast) : none(dy),
           need_w ? at::empty_like(*weight) : none(dy), need_b ? at::empty_like(*bias) : none(dy)};
 }
@@ -253,6 +270,7 @@ bool wants_grad(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& b
 }
 Tensor act_autograd(const Tensor& x, int64_t groups, const MaybeTensor& weight, const MaybeTensor& bias, double eps,
                     int64_t act, bool packed, bool checkpoint) {
+  refuse_tangents(x, weight, bias);
   if (!wants_grad(x, weight, bias)) {
     at::AutoDispatchBelowADInplaceOrView below;
     return std::get<0>(forward_op().call(x, groups, weight, bias, eps, act, packed, false, false));

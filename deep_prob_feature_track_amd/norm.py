@@ -73,7 +73,9 @@ def act_restore(c, dtype=None):
 
 def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="elu", packed=False, checkpoint=False):
     """act(group_norm(x)) of a map [N,C,H,W] in fp32, bf16 or fp16, channels_last (other layouts are
-    copied; the result is channels_last), differentiable once in x, weight and bias.
+    copied; the result is channels_last), differentiable once in x, weight and bias by the backward pass.
+    There is no forward-mode derivative: an input that carries a tangent raises NotImplementedError, and of
+    torch.func's transforms only vmap runs it (a call for each sample).
 
     groups divides C; weight / bias [C] (fp32 or another float type, both alike; None: 1 / 0); act
     'none', 'relu', 'elu' or 'silu'.
