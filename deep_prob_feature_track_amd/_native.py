@@ -7,6 +7,7 @@ load, every call raises.
 """
 import ctypes
 import os
+import struct
 
 import torch  # (must be imported before the HIP library, see above)
 
@@ -69,6 +70,21 @@ EXPORTS = ("dpft_workspace_size", "dpft_ic_solve_level", "dpft_ic_solve_pyramid"
 _lib = None
 
 
+def _check_whole(path):
+    """Raises OSError for a file that does not hold what its ELF program headers say is loaded from it (a build or a
+    copy that was cut off): the loader would map it all the same, and the process end by SIGBUS."""
+    with open(path, "rb") as f:
+        head = f.read(64)
+        if len(head) < 64 or head[:4] != b"\x7fELF":
+            raise OSError(f"{path} is not a shared library (cut short?): build it again")
+        at, each, count = struct.unpack_from("<Q", head, 32)[0], *struct.unpack_from("<HH", head, 54)
+        f.seek(at)
+        table, size = f.read(each * count), os.path.getsize(path)
+    offsets = [struct.unpack_from("<QQQQ", table, i * each + 8) for i in range(count)] if len(table) == each * count else None
+    if offsets is None or any(offset + filesz > size for offset, _, _, filesz in offsets):
+        raise OSError(f"{path} is cut short ({size} bytes): build it again")
+
+
 def lib():
     """Load (once) and return the CDLL; raises if the native library is unavailable."""
     global _lib
@@ -76,6 +92,7 @@ def lib():
         return _lib
     if not os.path.exists(LIB_PATH):
         raise RuntimeError(f"{LIB_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
+    _check_whole(LIB_PATH)
     L = ctypes.CDLL(LIB_PATH, mode=ctypes.RTLD_GLOBAL)
     P = ctypes.POINTER
     vp, sz = ctypes.c_void_p, ctypes.c_size_t
@@ -164,5 +181,6 @@ def torch_ops():
     lib()
     if not os.path.exists(TORCH_LIB_PATH):
         raise RuntimeError(f"{TORCH_LIB_PATH} is missing: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
+    _check_whole(TORCH_LIB_PATH)
     torch.ops.load_library(TORCH_LIB_PATH)
     return torch.ops.dpft

@@ -12,8 +12,6 @@ has a workspace of its own, so that calls on several streams, and captured graph
 trace under torch.compile.  CPU tensors raise: the modules of models/submodules.py take the torch path
 for them.
 """
-import os
-
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -22,8 +20,13 @@ from .ic import _eager_only
 
 BLOCK = 32  # values that share a step in a checkpoint
 
-# loaded with the module, so that nothing is left to a traced call; without the library every call raises
-_ops = N.torch_ops() if os.path.exists(N.LIB_PATH) and os.path.exists(N.TORCH_LIB_PATH) else None
+# loaded with the module, so that nothing is left to a traced call.  A library that is missing or does not load (half
+# written, stale, of another torch) does not end the import, which the CPU's and batch norm's users need too: every
+# call then tries again and raises.
+try:
+    _ops = N.torch_ops()
+except (OSError, RuntimeError, AttributeError):
+    _ops = None
 
 
 def _op(name):
