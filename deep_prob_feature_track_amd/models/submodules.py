@@ -12,6 +12,7 @@ import math
 import torch
 import torch.nn as nn
 from torch.nn import init
+from torch.nn.modules import module as _nn_module
 
 from .. import _native as N
 from .. import ic
@@ -42,6 +43,13 @@ def _padding(kernel_size, dilation):
     return (kernel_size - 1) // 2 + dilation - 1
 
 
+def _listened(m):
+    """True where calling module m does more than its class's forward: hooks of its own or of every module (pruning,
+    weight norm and spectral norm rebuild the weight in one), or a function put in forward's place."""
+    return bool(m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks
+                or "forward" in m.__dict__ or _nn_module._has_any_global_hook())
+
+
 class ConvBlock(nn.Sequential):
     """conv [-> batchnorm] -> ELU, an nn.Sequential (the reference's state_dict keys).
     In eval mode on the GPU, outside autograd, the batchnorm and the ELU of a 2-D block
@@ -50,7 +58,8 @@ class ConvBlock(nn.Sequential):
     modules run in turn.
     With a GroupNorm, a channels_last map on the GPU goes through `norm.group_norm_act`, in
     training too; with `act_checkpoint` the backward pass then keeps the conv's input and output
-    in 8 bits (`norm.conv2d`, `group_norm_act(checkpoint=True)`): 2 bytes a value, not 8."""
+    in 8 bits (`norm.conv2d`, `group_norm_act(checkpoint=True)`): 2 bytes a value, not 8.
+    A module with hooks is called, and what it would have kept in 8 bits is kept in full."""
 
     act_checkpoint = False
 
@@ -61,13 +70,14 @@ class ConvBlock(nn.Sequential):
     def _group_conv(self, x):
         c = self[0]
         if (self.act_checkpoint and torch.is_grad_enabled() and type(c) is nn.Conv2d and c.padding_mode == 'zeros'
-                and not isinstance(c.padding, str) and x.dim() == 4 and x.dtype in N.TYPES):
+                and not isinstance(c.padding, str) and x.dim() == 4 and x.dtype in N.TYPES and not _listened(c)):
             return gn.conv2d(x, c.weight, c.bias, c.stride, c.padding, c.dilation, c.groups)
         return c(x)
 
     def _group_epilogue(self, y, packed=False):
         n = self[1]
-        if y.dim() != 4 or y.dtype not in N.TYPES or not y.is_contiguous(memory_format=torch.channels_last):
+        if (y.dim() != 4 or y.dtype not in N.TYPES or not y.is_contiguous(memory_format=torch.channels_last)
+                or _listened(n) or _listened(self[2])):
             return self[2](n(y))
         return gn.group_norm_act(y, n.num_groups, n.weight, n.bias, n.eps, "elu", packed=packed,
                                  checkpoint=self.act_checkpoint)

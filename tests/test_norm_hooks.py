@@ -1,0 +1,164 @@
+"""A block with group normalisation calls its modules where something listens to them: hooks fire, pre-hooks that
+rebuild a weight (pruning, weight norm, spectral norm) run, whichever path the block would take.  The decisions need
+no device: the fused calls are recorded in place of the kernels."""
+import pytest
+import torch
+import torch.nn as nn
+import torch.nn.functional as F
+from torch.nn.modules import module as nn_module
+from torch.nn.utils import prune
+
+from deep_prob_feature_track_amd.models import submodules
+from deep_prob_feature_track_amd.models.submodules import convLayer
+
+gpu = pytest.mark.gpu
+
+
+@pytest.fixture
+def fused(monkeypatch):
+    """The block's fused calls, recorded; the values are torch's own."""
+    calls = []
+
+    def conv2d(x, *a):
+        calls.append("conv2d")
+        return F.conv2d(x, *a)
+
+    def group_norm_act(y, groups, weight, bias, eps, act, packed=False, checkpoint=False):
+        calls.append("group_norm_act")
+        return F.elu(F.group_norm(y, groups, weight, bias, eps))
+    monkeypatch.setattr(submodules.gn, "conv2d", conv2d)
+    monkeypatch.setattr(submodules.gn, "group_norm_act", group_norm_act)
+    return calls
+
+
+def _block(seed=0):
+    torch.manual_seed(seed)
+    return convLayer(True, 8, 16, 3, norm="group", act_checkpoint=True).to(memory_format=torch.channels_last)
+
+
+def _run(blk, x):
+    """What forward() does with a device map."""
+    return blk._group_epilogue(blk._group_conv(x))
+
+
+def _x():
+    return torch.randn(2, 8, 6, 7).contiguous(memory_format=torch.channels_last)
+
+
+def test_without_hooks_the_fused_calls_run(fused):
+    _run(_block(), _x())
+    assert fused == ["conv2d", "group_norm_act"]
+
+
+REGISTER = {
+    "pre": lambda m, f: m.register_forward_pre_hook(lambda m, i: f()),
+    "post": lambda m, f: m.register_forward_hook(lambda m, i, o: f()),
+    "post_always": lambda m, f: m.register_forward_hook(lambda m, i, o: f(), always_call=True),
+    "backward_pre": lambda m, f: m.register_full_backward_pre_hook(lambda m, g: f()),
+    "backward": lambda m, f: m.register_full_backward_hook(lambda m, i, o: f()),
+}
+
+
+@pytest.mark.parametrize("kind", REGISTER)
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_a_hook_fires(fused, which, kind):
+    blk, seen = _block(), []
+    if kind.startswith("backward"):
+        blk[2].inplace = False  # (torch refuses these hooks around an operation in place)
+    handle = REGISTER[kind](blk[which], lambda: seen.append(which))
+    x = _x().requires_grad_(True)
+    _run(blk, x).sum().backward()
+    assert seen == [which]
+    # the other half stays fused
+    assert fused == (["group_norm_act"] if which == 0 else ["conv2d"])
+    handle.remove()
+    del fused[:]
+    _run(blk, x).sum().backward()
+    assert seen == [which] and fused == ["conv2d", "group_norm_act"]
+
+
+@pytest.mark.parametrize("register", [nn_module.register_module_forward_hook, nn_module.register_module_forward_pre_hook,
+                                      nn_module.register_module_full_backward_hook,
+                                      nn_module.register_module_full_backward_pre_hook])
+def test_a_hook_on_every_module_fires(fused, register):
+    blk, seen = _block(), []
+    blk[2].inplace = False
+    handle = register(lambda m, *a: seen.append(type(m)) and None)
+    try:
+        _run(blk, _x().requires_grad_(True)).sum().backward()
+    finally:
+        handle.remove()
+    assert sorted(t.__name__ for t in seen) == ["Conv2d", "ELU", "GroupNorm"] and not fused
+
+
+@pytest.mark.parametrize("how", ["prune", "weight_norm", "spectral_norm", "parametrize"])
+def test_a_rebuilt_weight_is_the_fresh_one(fused, how):
+    """The weight that the convolution uses follows its source after a step of it."""
+    blk = _block().to(memory_format=torch.contiguous_format)  # (torch prunes no other layout)
+    c = blk[0]
+    if how == "prune":
+        prune.l1_unstructured(c, "weight", amount=0.5)
+        source = c.weight_orig
+    elif how == "weight_norm":
+        torch.nn.utils.weight_norm(c)
+        source = c.weight_g
+    elif how == "spectral_norm":
+        torch.nn.utils.spectral_norm(c)
+        source = c.weight_orig
+    else:
+        torch.nn.utils.parametrizations.weight_norm(c)
+        source = c.parametrizations.weight.original0
+    x = _x()
+    _run(blk, x)
+    with torch.no_grad():
+        source.mul_(3.0) if how != "spectral_norm" else source.add_(torch.randn_like(source))
+    got = blk._group_conv(x)
+    blk[0].eval()  # (spectral norm takes a step of its own in training)
+    assert torch.equal(got, F.conv2d(x, c.weight, None, c.stride, c.padding))
+    got.sum().backward()
+    assert source.grad is not None and source.grad.any()
+    assert "conv2d" not in fused
+
+
+def test_a_replaced_forward_is_called(fused):
+    """What wraps a module by putting a function in its forward's place."""
+    for which in (0, 1, 2):
+        blk, seen = _block(), []
+        plain = blk[which].forward
+        blk[which].forward = lambda v: seen.append(which) or plain(v)
+        del fused[:]
+        _run(blk, _x())
+        assert seen == [which] and fused == (["group_norm_act"] if which == 0 else ["conv2d"])
+
+
+def test_packed_heads_with_a_hook_come_unpacked(fused):
+    blk, seen = _block(), []
+    blk[1].register_forward_hook(lambda m, i, o: seen.append(1))
+    with torch.no_grad():
+        y = blk._group_epilogue(blk[0](_x()), packed=True)
+    assert y.shape == (2, 16, 6, 7) and seen == [1] and not fused
+
+
+@gpu
+@pytest.mark.parametrize("which", [1, 2])
+def test_a_hooked_block_on_the_device(which):
+    """The modules' values with a hook, the kernels' without: the same up to their roundings."""
+    if not torch.cuda.is_available():
+        pytest.skip("no HIP device")
+    import norm_oracle as O
+    blk = _block().to("cuda:0")
+    y = torch.randn(2, 16, 9, 11, device="cuda:0").contiguous(memory_format=torch.channels_last)
+    r = O.Reference(y, blk[1].num_groups, blk[1].weight, blk[1].bias, blk[1].eps, "elu")
+    with torch.no_grad():
+        plain = blk._group_epilogue(y)
+        assert blk._group_epilogue(y, packed=True).dim() == 5
+        seen = []
+        blk[which].register_forward_hook(lambda m, i, o: seen.append(which))
+        hooked, packed = blk._group_epilogue(y), blk._group_epilogue(y, packed=True)
+    assert seen == [which, which] and packed.shape == y.shape and torch.equal(packed, hooked)
+    assert O.excess(plain, r.y, r.y_tol) <= 0
+    # (the modules' statistics are sums in fp32 of the group's 396 values, in an order of the library's own; their y is
+    # x a + (b - mean a), two roundings of at most 5 U more: 400 terms in a row cover both)
+    run = 400
+    loose = O.Reference(y, blk[1].num_groups, blk[1].weight, blk[1].bias, blk[1].eps, "elu", run=run)
+    assert O.excess(hooked, loose.y, loose.y_tol) <= 0
