@@ -78,7 +78,7 @@ class ConvBlock(nn.Sequential):
         n = self[1]
         if (y.dim() != 4 or y.dtype not in N.TYPES or not y.is_contiguous(memory_format=torch.channels_last)
                 or _listened(n) or _listened(self[2])):
-            return self[2](n(y))
+            return self[2](n(y)).to(y.dtype)  # (autocast runs torch's group norm in fp32; the kernels keep y's type)
         return gn.group_norm_act(y, n.num_groups, n.weight, n.bias, n.eps, "elu", packed=packed,
                                  checkpoint=self.act_checkpoint)
 
