@@ -1,5 +1,6 @@
 """The normalisation kernels on the CPU, their buffers between pages that fault (cpu_kernels/norm_bounds.cpp): no
-access out of range, no barrier that a thread misses, no result left unwritten, at sizes that reach every path."""
+access out of range, no barrier that a thread misses, no result left unwritten.  At these sizes a workgroup visits one
+block of a sample; test_norm_two_pass.py has those where it walks over several, and compares values."""
 import os
 import subprocess
 
