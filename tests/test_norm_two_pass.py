@@ -1,5 +1,6 @@
 """The two-pass normalisation kernels where a workgroup visits several blocks of a sample: on the CPU (the kernels in
-coroutines, cpu_kernels/norm_values.cpp) and on a MI355X (`-m gpu`) against 64 bits."""
+coroutines, cpu_kernels/norm_values.cpp) and on a MI355X (`-m gpu`) against 64 bits; and the edge cases of fp32 maps
+at sizes that the one-launch kernel does not take."""
 import math
 import os
 import re
@@ -32,6 +33,7 @@ WIDE = (330, 512, 12, 12, 1)       # channel quads in tiles of their own
 FEW = {"kStatsWorkgroups": 4, "kSumsWorkgroups": 4, "kApplyWorkgroups": 6, "kGradWorkgroups": 6}
 SMALL = [(2, 30, 31, 43, 5), (2, 32, 40, 64, 8), (2, 258, 9, 17, 129), (2, 7, 79, 83, 1), (2, 1030, 5, 8, 5),
          (2, 4, 131, 101, 1), (2, 6, 110, 77, 3), (1, 16, 80, 72, 8), (1, 36, 63, 64, 3), (1, 512, 12, 13, 1)]
+EDGES = [(2, 30, 30, 40, 5), (1, 32, 64, 80, 8)]  # (D % 4 != 0; more pixels than a workgroup holds)
 
 
 def _map(n, c, h, w, dtype, seed=0, offset=0.0, dev="cpu"):
@@ -94,6 +96,13 @@ def test_device_sizes_loop(binary, shape, dtype):
     assert not one_launch
     for what, (blocks, parts) in zip(PASSES, walks):
         assert blocks > parts or (shape == WIDE) != (what == PASSES[2]), (what, blocks, parts)
+
+
+@pytest.mark.parametrize("shape", EDGES)
+def test_edge_sizes_take_two_passes(binary, shape):
+    """... and those of the edge cases several records a sample, in fp32."""
+    walks, _, one_launch = _walk(binary, shape, F32)
+    assert not one_launch and walks[0][1] > 1 and walks[3][1] > 1
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -202,3 +211,125 @@ def test_channel_quads(shape):
     assert torch.equal(norm.group_norm_act(x, groups, wt, b, packed=True), ic.pack_features(y.contiguous()))
     r = O.Reference(x, groups, wt, b, 1e-5, "elu", run=_run(shape, F32))
     assert O.excess(y, r.y, r.y_tol) <= 0
+
+
+# ------------------------------------------------------------------ edge cases in fp32
+@gpu
+@pytest.mark.parametrize("shape", EDGES)
+@pytest.mark.parametrize("offset", [1e3, 1e4, -1e4])
+def test_far_mean(shape, offset):
+    """The statistics of values far from 0: taken from squares, 0.06 or 6 times the spread's square would be lost
+    (offset^2 U).  The bounds of norm_oracle with a mean that is off by 32 U of itself: a mean of 8 values in a row by
+    4.4 U, at most 9 joins over neighbours and 6 over lanes by U each.  A part's mean that is off by e changes the
+    squares about the whole's by 2 e |mean - part's mean| + e^2, of which the first comes to at most 2 e times the
+    spread: rstd is off by e rstd + (e rstd)^2 of itself."""
+    dev = _dev()
+    n, c, h, w, groups = shape
+    x = _map(n, c, h, w, F32, seed=4, offset=offset, dev=dev).requires_grad_(True)
+    wt, b = (p.requires_grad_(True) for p in _params(c, 4, dev=dev))
+    dy = _map(n, c, h, w, F32, seed=54, dev=dev)
+    y = norm.group_norm_act(x, groups, wt, b, act="silu")
+    dx, dw, db = torch.autograd.grad(y, (x, wt, b), dy)
+    r = O.Reference(x, groups, wt, b, 1e-5, "silu", dy)
+    far = 32 * O.U * abs(offset) * 1.01  # the mean's own error
+    rstd = r.rstd.repeat_interleave(c // groups, 1).view(n, c, 1, 1)
+    xhat = (x.detach().double() - r.mean.repeat_interleave(c // groups, 1).view(n, c, 1, 1)) * rstd
+    g = wt.detach().double().view(1, c, 1, 1).abs()
+    rstd_off = far * rstd + (far * rstd) ** 2  # of itself
+    off = far * rstd * (1 + rstd_off) + xhat.abs() * rstd_off  # of xhat
+    assert off.max() < 0.2  # (far below what a lost spread would do)
+    assert O.excess(y, r.y, r.y_tol + 1.1 * g * off) <= 0
+    # the slope's derivative is at most 1/2 for silu, the slope at most 1.1
+    d = dy.double().abs()
+    u_off = d * 0.5 * g * off
+    assert O.excess(db, r.dbias, 1.01 * r.dbias_tol + u_off.sum((0, 2, 3))) <= 0
+    w_off = u_off * (xhat.abs() + off) + 1.1 * d * off
+    assert O.excess(dw, r.dweight, 1.01 * r.dweight_tol + w_off.sum((0, 2, 3))) <= 0
+
+    def gmean(v):
+        return v.reshape(n, groups, -1).mean(2).repeat_interleave(c // groups, 1).view(n, c, 1, 1)
+    m2 = gmean(1.1 * d * g * (xhat.abs() + off))
+    dx_off = rstd * (g * u_off + gmean(g * u_off) + (xhat.abs() + off) * gmean(g * w_off) + off * m2)
+    dx_off = dx_off * (1 + rstd_off) + rstd_off * rstd * (1.1 * d * g + gmean(1.1 * d * g) + (xhat.abs() + off) * m2)
+    assert O.excess(dx, r.dx, r.dx_tol + dx_off) <= 0
+
+
+@gpu
+@pytest.mark.parametrize("shape", EDGES)
+def test_an_outlier(shape):
+    dev = _dev()
+    n, c, h, w, groups = shape
+    for at in ((0, 0), (h // 2, w // 3), (h - 1, w - 1)):
+        x = _map(n, c, h, w, F32, seed=5, dev=dev).clone(memory_format=torch.channels_last)
+        x[:, :, at[0], at[1]] = 1e4
+        y = norm.group_norm_act(x, groups, act="none")
+        r = O.Reference(x, groups, None, None, 1e-5, "none")
+        assert O.excess(y, r.y, r.y_tol) <= 0
+
+
+@gpu
+@pytest.mark.parametrize("shape", EDGES)
+def test_non_finite_values_stay_in_their_group(shape):
+    """... of their sample, forward and backward: y, dx, and the gradients of the group's own channels."""
+    dev = _dev()
+    n, c, h, w, groups = shape
+    d = c // groups
+    x = _map(n, c, h, w, F32, seed=6, dev=dev)
+    wt, b = (p.requires_grad_(True) for p in _params(c, 6, dev=dev))
+    dy = _map(n, c, h, w, F32, seed=56, dev=dev)
+
+    def step(x, ck):
+        x = x.detach().requires_grad_(True)
+        y = norm.group_norm_act(x, groups, wt, b, checkpoint=ck)
+        return (y.detach(),) + torch.autograd.grad(y, (x, wt, b), dy)
+    keep = torch.ones(n, c, h, w, dtype=torch.bool, device=dev)
+    keep[n - 1, d:2 * d] = False  # group 1 of the last sample
+    for ck in (False, True):
+        ref = step(x, ck)
+        for bad in (float("nan"), float("inf"), -float("inf")):
+            for px in ((3, 4), (h - 1, w - 1)):
+                z = x.clone(memory_format=torch.channels_last)
+                z[n - 1, 2 * d - 1, px[0], px[1]] = bad
+                y, dx, dw, db = step(z, ck)
+                assert y[~keep].isnan().all() and torch.equal(y[keep], ref[0][keep])
+                assert dx[~keep].isnan().all()
+                assert dw[d:2 * d].isnan().all()
+                others = torch.ones(c, dtype=torch.bool, device=dev)
+                others[d:2 * d] = False
+                if not ck:  # (a checkpoint's block of 32 values, NaN as a whole, reaches into other groups' gradients)
+                    assert torch.equal(dx[keep], ref[1][keep])
+                    assert torch.equal(dw[others], ref[2][others]) and torch.equal(db[others], ref[3][others])
+
+
+@gpu
+@pytest.mark.parametrize("shape", EDGES)
+def test_constant_group(shape):
+    """No spread: xhat = 0, y = act(bias), and a gradient that its own mean and xhat = 0 leave."""
+    dev = _dev()
+    n, c, h, w, groups = shape
+    x = torch.full((n, c, h, w), 3.25, device=dev).contiguous(memory_format=torch.channels_last).requires_grad_(True)
+    wt, b = (p.requires_grad_(True) for p in _params(c, 7, dev=dev))
+    dy = _map(n, c, h, w, F32, seed=57, dev=dev)
+    y = norm.group_norm_act(x, groups, wt, b)
+    r = O.Reference(x, groups, wt, b, 1e-5, "elu", dy)
+    assert O.excess(y, r.y, r.y_tol) <= 0
+    dx, dw, db = torch.autograd.grad(y, (x, wt, b), dy)
+    assert O.excess(dx, r.dx, r.dx_tol) <= 0 and O.excess(dw, r.dweight, r.dweight_tol * 1.01 + 1e-30) <= 0
+    assert O.excess(db, r.dbias, r.dbias_tol * 1.01) <= 0
+
+
+@gpu
+@pytest.mark.parametrize("shape", EDGES)
+def test_relu(shape):
+    """relu's slope jumps at 0: dy is 0 where z is within its own error of it."""
+    dev = _dev()
+    n, c, h, w, groups = shape
+    x = _map(n, c, h, w, F32, seed=8, dev=dev).requires_grad_(True)
+    wt, b = (p.requires_grad_(True) for p in _params(c, 8, dev=dev))
+    r = O.Reference(x, groups, wt, b, 1e-5, "relu")
+    dy = _map(n, c, h, w, F32, seed=58, dev=dev) * (r.z.abs() > 4 * r.z_tol)
+    y = norm.group_norm_act(x, groups, wt, b, act="relu")
+    r = O.Reference(x, groups, wt, b, 1e-5, "relu", dy)
+    dx, dw, db = torch.autograd.grad(y, (x, wt, b), dy)
+    assert O.excess(y, r.y, r.y_tol) <= 0 and O.excess(dx, r.dx, r.dx_tol) <= 0
+    assert O.excess(dw, r.dweight, r.dweight_tol * 1.01) <= 0 and O.excess(db, r.dbias, r.dbias_tol * 1.01) <= 0
