@@ -8,6 +8,7 @@ import torch.nn.functional as F
 from torch.nn.modules import module as nn_module
 from torch.nn.utils import prune
 
+import norm_oracle as O
 from deep_prob_feature_track_amd.models import submodules
 from deep_prob_feature_track_amd.models.submodules import convLayer
 
@@ -145,7 +146,6 @@ def test_a_hooked_block_on_the_device(which):
     """The modules' values with a hook, the kernels' without: the same up to their roundings."""
     if not torch.cuda.is_available():
         pytest.skip("no HIP device")
-    import norm_oracle as O
     blk = _block().to("cuda:0")
     y = torch.randn(2, 16, 9, 11, device="cuda:0").contiguous(memory_format=torch.channels_last)
     r = O.Reference(y, blk[1].num_groups, blk[1].weight, blk[1].bias, blk[1].eps, "elu")
@@ -162,3 +162,22 @@ def test_a_hooked_block_on_the_device(which):
     run = 400
     loose = O.Reference(y, blk[1].num_groups, blk[1].weight, blk[1].bias, blk[1].eps, "elu", run=run)
     assert O.excess(hooked, loose.y, loose.y_tol) <= 0
+
+
+@gpu
+@pytest.mark.parametrize("act_checkpoint", [False, True])
+def test_a_compiled_block_is_traced_whole(act_checkpoint):
+    """At inference, plain and into the solver's layout: no graph break (the question for hooks is traced too)."""
+    if not torch.cuda.is_available():
+        pytest.skip("no HIP device")
+    torch.manual_seed(1)
+    blk = convLayer(True, 8, 16, 3, norm="group", act_checkpoint=act_checkpoint).to("cuda:0")
+    blk = blk.to(memory_format=torch.channels_last)
+    x = torch.randn(2, 8, 9, 11, device="cuda:0").contiguous(memory_format=torch.channels_last)
+    with torch.no_grad():
+        for call in (blk.forward, blk.forward_packed):
+            fast = torch.compile(call, backend="aot_eager", fullgraph=True)
+            conv = blk[0](x)  # (two runs of a convolution may differ in a bit: its own bound, through the block)
+            tol = 4 * 72 * O.U * float(conv.abs().max()) * float((blk[1].weight.abs() / conv.std()).max())
+            got, want = fast(x), call(x)
+            assert got.shape == want.shape and (got - want).abs().max() <= tol
