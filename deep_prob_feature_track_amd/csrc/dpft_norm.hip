@@ -8,8 +8,10 @@
 // stay in registers.  A row that L cuts short is handled value by value.
 //
 // Everything here moves far more bytes than it computes on (12 to 40 flops per value of 2 to 20
-// bytes): HBM bound at the large sizes, launch bound at the small ones.  The figures beside the kernels
-// are of data that no cache holds; a copy of 1 GiB reaches 5.15 TB/s (read and written) on the same card.
+// bytes): bound by memory at the large sizes, by launches at the small ones.  The rates beside the kernels
+// are the bytes that they ask for over their time, in graphs of calls on many sets of inputs: a call's inputs
+// come from HBM, and of what a second pass reads again the Infinity Cache still holds a part, which is why some
+// exceed the 6.22 TB/s (read and written) of dpft_copy_probe on 1 GiB.
 // Two passes over x, not one: kernels that held a sample's values in registers from the statistics to
 // the result, workgroups waiting for each other's sums, took 198 to 303 us where two passes took 213 to
 // 291 -- all of them load, join and store at the same time, and the memory idles in between.
@@ -204,7 +206,7 @@ __device__ __forceinline__ void restore_vec(typename Bytes<V>::type b, float ste
 }
 
 // 16 bytes of x per thread and step, kUnroll steps in flight; the block's maximum by lane shifts.
-// Bound by HBM (8 x 32 x 480 x 640 fp32: 64 us, 6.2 TB/s).
+// Bound by memory (8 x 32 x 480 x 640 fp32: 64 us, 6.2 TB/s).
 constexpr int kUnroll = 4;
 template <typename T>
 __global__ __launch_bounds__(kThreads) void act_checkpoint_kernel(const T* __restrict__ x, int64_t n,
@@ -375,7 +377,7 @@ __device__ __forceinline__ void over_entries(const Walk& w, int tile, int V, int
 // Records [n][parts * tiles][G]: mean, sum of squares about it and count of the workgroup's values of a
 // group.  A thread takes the exact mean of kDeep values of a position, then their squares about it, and
 // joins the batches by the parallel-variance rule; the threads are joined in the same way: nothing
-// cancels, whatever the mean is.  Bound by HBM: 8 x 32 x 480 x 640 fp32 53.0 us, 5.9 TB/s; 16 x 64 x
+// cancels, whatever the mean is.  Bound by memory: 8 x 32 x 480 x 640 fp32 53.0 us, 5.9 TB/s; 16 x 64 x
 // 240 x 320 bf16 30.7 us, 5.1 TB/s.
 template <typename T>
 __global__ __launch_bounds__(kThreads) void gn_stats_kernel(const T* __restrict__ x, Walk w, float4* __restrict__ rec) {
@@ -533,7 +535,7 @@ struct Affine {
 // y = act((x - mean) a + bias), a = rstd * weight.
 // MODE: y as x is stored, in the channel-quad layout, or with x's checkpoint (w.lanes_block).
 // rec: the workgroup joins the statistics itself (kFold groups at most), its part 0 stores them.
-// Bound by HBM: 8 x 32 x 480 x 640 fp32 100.6 us, 6.3 TB/s; 16 x 64 x 240 x 320 bf16 52.9 us, 5.9; with
+// Bound by memory: 8 x 32 x 480 x 640 fp32 100.6 us, 6.3 TB/s; 16 x 64 x 240 x 320 bf16 52.9 us, 5.9; with
 // a checkpoint, 8 x 64 x 240 x 320 fp32 64.4 us, 5.5.
 constexpr int kFold = 128;
 enum { kPlain, kPacked, kCheckpoint };
@@ -866,7 +868,7 @@ struct Coefs {
 };
 
 // With g = dy act'(z): per (sample, part, position of a row) sum g and sum g xhat, and per (sample,
-// part, tile, group) sum weight g and sum weight g xhat.  Bound by HBM: 16 x 64 x 240 x 320 bf16 53.6 us,
+// part, tile, group) sum weight g and sum weight g xhat.  Bound by memory: 16 x 64 x 240 x 320 bf16 53.6 us,
 // 5.9 TB/s; from a checkpoint, 8 x 64 x 240 x 320 fp32 41.2 us, 4.8.
 template <typename T, int ACT, bool Q8>
 __global__ __launch_bounds__(kThreads) void gn_grad_sums_kernel(const T* __restrict__ dy, Source<T, Q8> x, Walk w,
@@ -1040,7 +1042,7 @@ __global__ __launch_bounds__(kThreads) void gn_param_grads_kernel(Params pg, int
   param_grads(pg.pos, pg.rows, C, type, pg.dweight, pg.dbias, blockIdx.x);
 }
 
-// dx = a g - rstd E[weight g] - (x - mean) rstd^2 E[weight g xhat], a = rstd * weight.  Bound by HBM:
+// dx = a g - rstd E[weight g] - (x - mean) rstd^2 E[weight g xhat], a = rstd * weight.  Bound by memory:
 // 16 x 64 x 240 x 320 bf16 79.6 us, 5.9 TB/s; from a checkpoint, 8 x 64 x 240 x 320 fp32 59.8 us, 5.9.
 template <typename T, int ACT, bool Q8>
 __global__ __launch_bounds__(kThreads) void gn_grad_input_kernel(const T* __restrict__ dy, Source<T, Q8> x, Walk w,

@@ -71,7 +71,8 @@ class FeaturePyramid(nn.Module):
     recognises and hands to the kernel as one plane (Cs = 1: 2 sigma planes of reads
     per pixel instead of 2C).
     norm='group': group normalisation in every block instead of batch normalisation;
-    act_checkpoint (with it): a training step on the GPU keeps the blocks' activations in 8 bits."""
+    act_checkpoint (with it): a training step on the GPU keeps the blocks' activations in 8 bits; needs the module and
+    its input in channels_last (the tracker sees to both)."""
 
     def __init__(self, D, w_uncertainty='None', feature_channel=1, feature_extract='conv', uncertainty_channel=1,
                  norm='batch', act_checkpoint=False):

@@ -56,7 +56,7 @@ class ConvBlock(nn.Sequential):
     run as one in-place pass over the conv output (`ic.bn_elu_`, dpft_bn_elu) instead of
     two elementwise kernels; otherwise, or for a layout the kernel does not take, the
     modules run in turn.
-    With a GroupNorm, a channels_last map on the GPU goes through `norm.group_norm_act`, in
+    With a GroupNorm, a channels_last map (fp32, bf16, fp16) on the GPU goes through `norm.group_norm_act`, in
     training too; with `act_checkpoint` the backward pass then keeps the conv's input and output
     in 8 bits (`norm.conv2d`, `group_norm_act(checkpoint=True)`): 2 bytes a value, not 8.
     A module with hooks is called, and what it would have kept in 8 bits is kept in full."""
@@ -140,7 +140,8 @@ _NORMS = {'batch': nn.BatchNorm2d, 'group': group_norm}
 
 def convLayer(batchNorm, in_planes, out_planes, kernel_size=3, stride=1, dilation=1, bias=False, norm='batch',
               act_checkpoint=False):
-    """Conv2d [+ BatchNorm2d, or GroupNorm with norm='group'] + ELU; act_checkpoint (group norm only): ConvBlock."""
+    """Conv2d [+ BatchNorm2d, or GroupNorm with norm='group'] + ELU; act_checkpoint (group norm only): ConvBlock, whose
+    weights must be channels_last (with other maps the convolution's input alone is kept in 8 bits)."""
     if norm not in _NORMS:
         raise ValueError(f"norm must be one of {sorted(_NORMS)} (got {norm!r})")
     if act_checkpoint and (norm != 'group' or not batchNorm):

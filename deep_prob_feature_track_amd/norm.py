@@ -61,7 +61,9 @@ def act_checkpoint(x):
     """x (fp32, bf16 or fp16, any shape) in 8 bits -> ActCheckpoint.  Values go in blocks of 32 in
     memory order (a channels_last map: along its channels), each block with a step of 2^(E - 6) where
     2^E <= max |x| < 2^(E + 1): off by at most half a step, max |x| / 128 and less (a whole step where
-    127 steps clamp the largest).  A block with an infinity or a NaN restores as NaN."""
+    127 steps clamp the largest).  A block with an infinity or a NaN restores as NaN.
+    Outside autograd: no gradient and no tangent goes through.  A traced call runs it eagerly (a graph break;
+    fullgraph=True raises), as act_restore and conv2d."""
     x = _dense(x.detach())
     q, scale = _op("act_checkpoint")(x)
     return ActCheckpoint(q, scale, x.shape, x.stride(), x.dtype)
@@ -123,7 +125,8 @@ def _pair(v):
 @_eager_only
 def conv2d(x, weight, bias=None, stride=1, padding=0, dilation=1, groups=1):
     """torch.nn.functional.conv2d whose backward pass keeps x as an 8-bit checkpoint: the same y and
-    gradient of x, the weight's gradient at the restored x.  Under autocast, in its dtype."""
+    gradient of x, the weight's gradient at the restored x.  Under autocast, in its dtype.  Not covered by a running
+    test with the device library's own convolution gradients (the CPU's are, and what the device's are handed)."""
     if isinstance(padding, str):
         raise ValueError(f"padding must be numbers (got {padding!r})")
     if not x.is_cuda:

@@ -324,6 +324,9 @@ int dpft_bn_elu_pack(const float* x, const float* chan, float* out, int32_t B, i
  *                                dx = rstd (weight g - E[weight g] - xhat E[weight g xhat]).
  * The workspace needs no initialisation and holds nothing between calls; one call at a time
  * may use it.  x / y / dy / dx are 16-byte aligned and not aliased.
+ * Sizes: C <= 2^20, pixels * C <= 2^40, N * (C / 256 + 1) <= 2^20, N * C <= 2^30; others are refused.
+ * From a checkpoint, a block of 32 values that holds a non-finite one is NaN as a whole, and with it the
+ * gradients of every group and channel that it reaches into.
  */
 #define DPFT_TYPE_F32  0
 #define DPFT_TYPE_BF16 1

@@ -4,6 +4,7 @@ eager and in the variants `models.LeastSquareTracking` may choose between, and p
 per-kernel breakdown of the NCHW and channels_last calls.
 
 python tools/encoder_timing.py [--batch 16] [--reps 20]
+python tools/encoder_timing.py --norm group   # group normalisation: the fused blocks beside the modules in turn
 """
 import argparse
 import copy
@@ -22,11 +23,12 @@ ap.add_argument("--batch", type=int, default=16, help="frames (2 per pair)")
 ap.add_argument("--reps", type=int, default=20)
 ap.add_argument("--down", type=int, default=1)
 ap.add_argument("--channels", type=int, default=32)
+ap.add_argument("--norm", choices=("batch", "group"), default="batch")
 a = ap.parse_args()
 dev = torch.device("cuda:0")
 torch.manual_seed(0)
 enc = FeaturePyramid(D=8, w_uncertainty="laplacian", feature_channel=a.channels, feature_extract="conv",
-                     uncertainty_channel=1).to(dev).eval()
+                     uncertainty_channel=1, norm=a.norm).to(dev).eval()
 H, W = 480 // a.down, 640 // a.down
 x = torch.randn(a.batch, 8, H, W, device=dev)
 
@@ -53,7 +55,20 @@ def max_rel(ref, out):
 with torch.no_grad():
     ref = enc(x)
 base = timed(enc, x)
-print(f"encoder B={a.batch} {W}x{H} C={a.channels}: eager {base:.2f} ms", flush=True)
+print(f"encoder B={a.batch} {W}x{H} C={a.channels} norm={a.norm}: eager {base:.2f} ms", flush=True)
+if a.norm == "group":
+    from deep_prob_feature_track_amd.models import submodules
+    cl = copy.deepcopy(enc).to(memory_format=torch.channels_last)
+    xc = x.contiguous(memory_format=torch.channels_last)
+    fused = submodules.ConvBlock._group
+    for name, rule, kw in (("fused", fused, {}), ("fused, heads in the solver's layout", fused, dict(packed=True)),
+                           ("the modules in turn", lambda self, x: False, {})):
+        submodules.ConvBlock._group = rule
+        with torch.no_grad():
+            out = cl(xc, **kw)
+        rel = "" if kw else f", max rel diff {max_rel(ref, out):.2e}"
+        print(f"  channels_last, {name}: {timed(lambda t: cl(t, **kw), xc):.2f} ms{rel}", flush=True)
+    sys.exit()
 
 def fold_bn(mod):
     """conv -> batchnorm (eval) folded into one conv with bias (rounding differs)."""
