@@ -73,7 +73,7 @@ def binary(tmp_path_factory):
     (folder / "norm_bounds.cpp").write_text(bounds.replace(include, '#include "dpft_norm.hip"'))
     (folder / "norm_values.cpp").write_text(open(os.path.join(HERE, "cpu_kernels", "norm_values.cpp")).read())
     out = str(folder / "norm_values")
-    subprocess.run([CLANG, "-x", "c++", "-std=c++17", "-O1", "-w", f"-I{HERE}/cpu_kernels", f"-I{B.INC}", f"-I{B.CSRC}",
+    subprocess.run([CLANG, "-x", "c++", "-std=c++17", "-O0", "-w", f"-I{HERE}/cpu_kernels", f"-I{B.INC}", f"-I{B.CSRC}",
                     str(folder / "norm_values.cpp"), "-o", out], check=True)
     return out
 
